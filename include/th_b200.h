@@ -304,6 +304,105 @@ typedef struct {
 } th_allreduce_args;
 int th_allreduce(const th_allreduce_args* a, void* stream);
 
+/* -------------------------------------------------------------------- rope
+ * Rotary positions.  Pair i (0 <= i < rotary_dim / 2) of every head of token
+ * t turns by the angle of row positions[t] of the tables:
+ *   (a, b) -> (a*c - b*s, a*s + b*c),  c = cos[positions[t], i], s = sin[...]
+ * where (a, b) are elements (i, i + rotary_dim/2) of the head, or with
+ * `interleaved` elements (2i, 2i+1); elements from rotary_dim on pass through.
+ * `inverse` turns by the opposite angle: the gradient of the rotation (for
+ * tables that carry a factor, the factor is kept, as its gradient does).
+ * Products and sums in fp32, one rounding at the end.  cos / sin are fp32
+ * [table_rows, rotary_dim/2] at ld_cs.  q and k are addressed by a token and
+ * a head stride in elements, with unit element stride; either may be NULL
+ * with 0 heads.  An output may be its input (same pointer and strides); they
+ * may not overlap in any other way.  A negative position marks a padding
+ * token: its outputs are zero.  A position >= table_rows sets
+ * TH_DEVERR_BAD_ARG in the device error word and also gives zeros. */
+typedef struct {
+  const void* q;      int64_t q_token, q_head;
+  void* q_out;        int64_t qo_token, qo_head;
+  const void* k;      int64_t k_token, k_head;
+  void* k_out;        int64_t ko_token, ko_head;
+  const int32_t* positions;                      /* [tokens] */
+  const float* cos;
+  const float* sin;   int64_t ld_cs;
+  int64_t tokens;
+  int32_t table_rows, hq, hkv, head_dim, rotary_dim, interleaved, inverse, dtype;
+  /* th_rope_append only: values, the page pools and the page table */
+  const void* v;      int64_t v_token, v_head;
+  void* k_pages;      int64_t k_page, k_phead, k_slot;
+  void* v_pages;      int64_t v_page, v_phead, v_slot;
+  const int32_t* table; int64_t ld_table;        /* [batch, table_cols] page ids */
+  const int32_t* seqs;                           /* [tokens] row of table; NULL: token t is row t */
+  int32_t batch, table_cols, page_size, num_pages;
+} th_rope_args;
+int th_rope(const th_rope_args* a, void* stream);
+
+/* ------------------------------------------------------------- rope_append
+ * th_rope on q, and into a paged key-value cache: the rotated k and the
+ * unrotated v of token t are stored at slot positions[t] % page_size of page
+ * table[seqs[t], positions[t] / page_size] (page, head and slot strides in
+ * elements, unit element stride; the pools' layouts may differ).  q may be
+ * NULL with hq = 0.  `inverse` is not used; k_out, when given, receives the
+ * rotated keys as well (a prompt's own attention reads them there).  Two
+ * tokens of one call must not name the same slot.  A padding token (negative position) stores
+ * nothing; a seqs entry, a table column or a page id out of range sets
+ * TH_DEVERR_BAD_ARG and stores nothing (q is still rotated). */
+int th_rope_append(const th_rope_args* a, void* stream);
+
+/* --------------------------------------------------------- paged_attention
+ * Attention of one new token per sequence over the paged cache:
+ *   s_j = scale * q.k_j, with softcap > 0: s_j = softcap * tanh(s_j / softcap)
+ *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j
+ * over keys j < lens[b] (the new token's own key is the last one), with
+ * window > 0 only the last `window` of them.  Key j of sequence b is slot
+ * j % page_size of page table[b, j / page_size].  Query head h reads
+ * key-value head h / (hq/hkv).  lens[b] <= 0 gives zeros (and lse = -inf).
+ * lse, when given, is log sum_j exp(s_j), fp32 [batch, hq] contiguous.
+ * Scores, maxima, sums and accumulators are fp32.  A page id out of range,
+ * or a length beyond table_cols * page_size, sets TH_DEVERR_BAD_ARG and
+ * drops the keys concerned.  head_dim * element size must be a multiple of
+ * 16 bytes (head_dim <= 256), the pools 16-byte aligned in base and strides.
+ * The workspace (th_paged_attention_workspace_size bytes, 16-byte aligned)
+ * must be zero before its first use; every call leaves its counters at zero,
+ * so it can be kept.  Calls that share one must not overlap on the GPU. */
+typedef struct {
+  const void* q;        int64_t q_row, q_head;
+  void* o;              int64_t o_row, o_head;
+  float* lse;
+  const void* k_pages;  int64_t k_page, k_head, k_slot;
+  const void* v_pages;  int64_t v_page, v_head, v_slot;
+  const int32_t* table; int64_t ld_table;
+  const int32_t* lens;
+  int32_t batch, hq, hkv, head_dim, page_size, num_pages, table_cols, window;
+  float scale, softcap;
+  int32_t dtype;
+  void* workspace;
+  size_t workspace_bytes;
+} th_paged_attention_args;
+size_t th_paged_attention_workspace_size(int32_t hq, int32_t hkv, int32_t head_dim, int32_t dtype);
+int th_paged_attention(const th_paged_attention_args* a, void* stream);
+
+/* --------------------------------------------------------------- page_copy
+ * Copies pages of a pool [num_pages, planes, page_size, width] (width
+ * contiguous bytes per slot, slots contiguous; page and plane strides in
+ * bytes): for every pair i, slots [0, counts[i]) of every plane of page
+ * src[i] go to page dst[i] (counts NULL: all slots).  Forks copy the last,
+ * partly filled page; compaction moves whole pages.  A negative src or dst
+ * skips the pair.  Destinations must be distinct and none may be a source of
+ * the same call.  An id or count out of range sets TH_DEVERR_BAD_ARG and
+ * skips the pair. */
+typedef struct {
+  void* pages;
+  int64_t page_stride, plane_stride, slot_bytes;
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* counts;
+  int32_t pairs, num_pages, planes, page_size;
+} th_page_copy_args;
+int th_page_copy(const th_page_copy_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,563 @@
+"""Rotary positions, the paged cache's attention and page copies on the GPU, each against a plain statement in
+64 bits.
+
+Bounds on rel-L2, with u = 2^-p the largest relative rounding of a p-bit output (8 bits bf16, 11 fp16, 24 fp32):
+* rope: u + 2^-22 (two 32-bit products and their sum, over tables both sides share);
+* attention: u + 1e-5: a 32-bit score of d = 128 products with |q||k| scale of about 17 errs by about
+  sqrt(128) 2^-24 17 = 1e-5, and weights kept to 16 bits or better add 2^-17;
+* page copies and stored values: equal bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from conftest import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def L():
+    from torch_helion.b200 import lib
+
+    lib.load()
+    lib.device_error()
+    return lib
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(L):
+    yield
+    torch.cuda.synchronize()
+    assert L.device_error() == 0
+
+
+def rand(*shape, dtype=torch.float32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g, device="cuda")).to(dtype)
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# -------------------------------------------------------------------- rope
+def rope64(x, pos, cos, sin, interleaved=False, inverse=False):
+    """Rows of the rotation matrix, pair by pair, in 64 bits; a negative position gives zeros."""
+    x, half = x.double().clone(), cos.shape[1]
+    c, s = cos.double()[pos.long().clamp(min=0)][:, None], sin.double()[pos.long().clamp(min=0)][:, None]
+    s = -s if inverse else s
+    ia = torch.arange(half, device=x.device) * (2 if interleaved else 1)
+    ib = ia + (1 if interleaved else half)
+    a, b = x[..., ia].clone(), x[..., ib].clone()
+    x[..., ia], x[..., ib] = a * c - b * s, a * s + b * c
+    return x * (pos >= 0)[:, None, None]
+
+
+def tables(L, rows, rotary):
+    from torch_helion.b200.kv_cache import rope_tables
+
+    return rope_tables(rows, rotary, 10000.0, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("tokens,hq,hkv,d,rotary", [(1, 32, 8, 128, 128), (37, 8, 8, 64, 48), (513, 5, 1, 80, 80),
+                                                    (3, 3, 2, 14, 6), (64, 1, 1, 256, 32), (130, 20, 1, 96, 96)])
+def test_rope(L, dtype, interleaved, inverse, tokens, hq, hkv, d, rotary):
+    q, k = rand(tokens, hq, d, dtype=dtype), rand(tokens, hkv, d, dtype=dtype, seed=1)
+    cos, sin = tables(L, 1000, rotary)
+    pos = torch.randint(0, 1000, (tokens,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).int()
+    pos[tokens // 2] = -1 if tokens > 1 else 999
+    qo, ko = L.rope(q, k, pos, cos, sin, interleaved=interleaved, inverse=inverse)
+    for x, got in ((q, qo), (k, ko)):
+        assert rel_l2(got, rope64(x, pos, cos, sin, interleaved, inverse)) <= U[dtype] + 2**-22
+        assert torch.equal(got[..., rotary:][pos >= 0], x[..., rotary:][pos >= 0])
+        assert bool((got[pos < 0] == 0).all())
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("offset", [0, 1, 8])
+def test_rope_strides_and_in_place(L, interleaved, offset):
+    """q and k inside one projection with a padded row, at an even, an odd and a 16-byte element offset; outputs in
+    place and head-major."""
+    t, hq, hkv, d = 45, 6, 2, 64
+    base = rand(t, (hq + 2 * hkv) * d + 24, dtype=torch.bfloat16)
+    flat = base[:, offset : offset + (hq + 2 * hkv) * d]
+    q = flat[:, : hq * d].unflatten(1, (hq, d))
+    k = flat[:, hq * d : (hq + hkv) * d].unflatten(1, (hkv, d))
+    cos, sin = tables(L, 64, d)
+    pos = torch.arange(t, device="cuda", dtype=torch.int32)
+    want_q, want_k = rope64(q, pos, cos, sin, interleaved), rope64(k, pos, cos, sin, interleaved)
+    before = base.clone()
+    head_major = torch.empty(hq, t, d, dtype=q.dtype, device="cuda").transpose(0, 1)
+    L.rope(q, k, pos, cos, sin, q_out=head_major, k_out=k, interleaved=interleaved)
+    assert rel_l2(head_major, want_q) <= U[q.dtype] + 2**-22 and rel_l2(k, want_k) <= U[q.dtype] + 2**-22
+    k.copy_(before[:, offset + hq * d : offset + (hq + hkv) * d].unflatten(1, (hkv, d)))
+    assert torch.equal(base, before)  # nothing beside k was touched
+    alone, none = L.rope(q, None, pos, cos, sin, interleaved=interleaved)
+    assert none is None and torch.equal(alone, head_major)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_gradient(L, interleaved):
+    """inverse=True is the vector-Jacobian product: against autograd of the 64-bit form, and against central
+    differences of the kernel itself (the rotation is linear, so a step of 1 has no truncation error; sums of
+    7 x 2 x 64 products of order 1 in 32 bits err by less than 1e-4)."""
+    t, h, d, r = 7, 2, 64, 48
+    cos, sin = tables(L, 64, r)
+    pos = ints([3, 0, 63, 8, 8, 1, 40])
+    x, g = rand(t, h, d), rand(t, h, d, seed=5)
+    got, _ = L.rope(g, None, pos, cos, sin, interleaved=interleaved, inverse=True)
+    xd = x.double().requires_grad_()
+    (rope64(xd, pos, cos, sin, interleaved) * g.double()).sum().backward()
+    assert rel_l2(got, xd.grad) <= 2**-22
+    for seed in range(4):
+        e = rand(t, h, d, seed=10 + seed)
+        up, _ = L.rope(x + e, None, pos, cos, sin, interleaved=interleaved)
+        down, _ = L.rope(x - e, None, pos, cos, sin, interleaved=interleaved)
+        slope = float(((up.double() - down.double()) * g.double()).sum()) / 2
+        assert abs(slope - float((got.double() * e.double()).sum())) < 1e-4
+
+
+def test_rope_position_beyond_the_tables(L):
+    q = rand(4, 2, 64, dtype=torch.bfloat16)
+    cos, sin = tables(L, 16, 64)
+    pos = ints([0, 16, 15, 2**31 - 1])
+    out, _ = L.rope(q, None, pos, cos, sin)
+    assert L.device_error() != 0  # reported, and cleared by the read
+    assert bool((out[[1, 3]] == 0).all()) and rel_l2(out[[0, 2]], rope64(q[[0, 2]], pos[[0, 2]], cos, sin)) <= U[q.dtype] + 2**-22
+
+
+# ------------------------------------------------------------------ append
+def pools(n, hkv, page, d, dtype, layout, seed=3):
+    """(keys, values) pools whose layouts differ in memory: heads first or slots first inside a page."""
+    def one(s):
+        if layout == "slots":
+            return rand(n, page, hkv, d, dtype=dtype, seed=s).transpose(1, 2)
+        return rand(n, hkv, page, d, dtype=dtype, seed=s)
+
+    if layout == "planes":
+        both = rand(n, 3, 2, hkv, page, d, dtype=dtype, seed=seed)
+        return both[:, 1, 0], both[:, 1, 1]
+    return one(seed), one(seed + 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["heads", "slots", "planes"])
+@pytest.mark.parametrize("hq,hkv,d,rotary,page,interleaved", [(32, 8, 128, 128, 16, False), (6, 2, 80, 40, 24, True),
+                                                              (0, 1, 64, 64, 1, False), (5, 5, 12, 4, 7, False)])
+def test_rope_append(L, dtype, layout, hq, hkv, d, rotary, page, interleaved):
+    lens, new = [0, page - 1, page, 3 * page + 1, 40], [3, 1, 2, page + 2, 0]
+    cols = max(-(-(n + m) // page) for n, m in zip(lens, new))
+    n_pages = 5 * cols + 2
+    kp, vp = pools(n_pages, hkv, page, d, dtype, layout)
+    table = torch.randperm(n_pages, device="cuda")[: 5 * cols].int().view(5, cols)
+    pos = ints([n + i for n, m in zip(lens, new) for i in range(m)] + [-1])
+    seqs = ints([s for s, m in enumerate(new) for _ in range(m)] + [2])
+    t = pos.shape[0]
+    qkv = rand(t, hq + 2 * hkv, d, dtype=dtype)
+    q, k, v = qkv[:, :hq], qkv[:, hq : hq + hkv], qkv[:, hq + hkv :]
+    cos, sin = tables(L, 200, rotary)
+    want_k, want_v = kp.clone(), vp.clone()
+    turned = rope64(k, pos, cos, sin, interleaved)
+    touched = torch.zeros(n_pages, page, dtype=torch.bool, device="cuda")
+    for i in range(t - 1):
+        page_id, slot = int(table[seqs[i], pos[i] // page]), int(pos[i] % page)
+        want_v[page_id, :, slot] = v[i]
+        touched[page_id, slot] = True
+        want_k[page_id, :, slot] = turned[i].to(dtype)
+    k_out = torch.empty(t, hkv, d, dtype=dtype, device="cuda")
+    got = L.rope_append(q if hq else None, k, v, pos, cos, sin, kp, vp, table, seqs=seqs, interleaved=interleaved, k_out=k_out)
+    assert torch.equal(vp, want_v)
+    at = touched[:, None, :, None].expand_as(kp)
+    assert torch.equal(kp[~at], want_k[~at]) and rel_l2(kp[at], want_k[at]) <= 2 * U[dtype] + 2**-22
+    assert rel_l2(k_out, turned) <= U[dtype] + 2**-22
+    if hq:
+        assert rel_l2(got, rope64(q, pos, cos, sin, interleaved)) <= U[dtype] + 2**-22
+    else:
+        assert got is None
+
+
+def test_rope_append_one_token_each_and_bad_ids(L):
+    """Without seqs token t is row t.  Ids out of range are reported, and nothing is stored for them."""
+    kp, vp = pools(6, 2, 8, 64, torch.bfloat16, "heads")
+    k, v, q = (rand(4, h, 64, dtype=torch.bfloat16, seed=h + 7) for h in (2, 2, 4))
+    v = rand(4, 2, 64, dtype=torch.bfloat16, seed=30)
+    cos, sin = tables(L, 100, 64)
+    before = kp.clone(), vp.clone()
+    table = ints([[0, 6], [-1, 1], [2, 3], [4, 5]])
+    pos = ints([9, 3, 16, 15])  # page id 6 of 6; page id -1; column 2 of 2; fine
+    out = L.rope_append(q, k, v, pos, cos, sin, kp, vp, table)
+    assert L.device_error() != 0
+    assert rel_l2(out, rope64(q, pos, cos, sin)) <= U[q.dtype] + 2**-22
+    before[0][5, :, 7], before[1][5, :, 7] = kp[5, :, 7], v[3]
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+    assert rel_l2(kp[5, :, 7], rope64(k, pos, cos, sin)[3]) <= U[q.dtype] + 2**-22
+    L.rope_append(None, k, v, ints([0, 0, 0, 0]), cos, sin, kp, vp, table, seqs=ints([-1, 4, 5, 2**31 - 1]))
+    assert L.device_error() != 0 and torch.equal(kp, before[0])
+
+
+# --------------------------------------------------------------- attention
+def attend64(q, kp, vp, table, lens, scale, softcap=0.0, window=0):
+    """Sequence by sequence in 64 bits: (outputs, log sums of exponentials)."""
+    b, hq, d = q.shape
+    hkv, page = kp.shape[1], kp.shape[2]
+    out = torch.zeros(b, hq, d, dtype=torch.float64, device=q.device)
+    lse = torch.full((b, hq), float("-inf"), dtype=torch.float64, device=q.device)
+    for i, n in enumerate(lens.tolist()):
+        if n <= 0:
+            continue
+        j = torch.arange(max(0, n - window) if window else 0, n, device=q.device)
+        ids = table[i, j // page].long()
+        k, v = kp[ids, :, j % page].double(), vp[ids, :, j % page].double()  # [n, hkv, d]
+        x = torch.einsum("hgd,nhd->hgn", q[i].double().view(hkv, hq // hkv, d), k) * scale
+        if softcap:
+            x = softcap * torch.tanh(x / softcap)
+        out[i] = torch.einsum("hgn,nhd->hgd", torch.softmax(x, -1), v).reshape(hq, d)
+        lse[i] = torch.logsumexp(x, -1).reshape(hq)
+    return out, lse
+
+
+def cached(lens, hkv, d, page, dtype, layout="heads", seed=11, poison=True):
+    """Pools, table and lengths; every slot past a sequence's end and every unused page holds NaN."""
+    need = [max(0, -(-n // page)) for n in lens]
+    cols, n_pages = max(1, max(need)) + 1, sum(need) + 2
+    kp, vp = pools(n_pages, hkv, page, d, dtype, layout, seed=seed)
+    order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(seed)).int()
+    table = torch.full((len(lens), cols), -1, dtype=torch.int32)
+    at, used = 0, torch.zeros(n_pages, page, dtype=torch.bool)
+    for i, (n, m) in enumerate(zip(lens, need)):
+        table[i, :m] = order[at : at + m]
+        for c in range(m):
+            used[order[at + c], : min(page, n - c * page)] = True
+        at += m
+    if poison:
+        mask = ~used.cuda()[:, None, :, None].expand_as(kp)
+        kp[mask], vp[mask] = float("nan"), float("nan")
+    return kp, vp, table.cuda(), ints(lens)
+
+
+def check_attend(L, q, kp, vp, table, lens, bound=None, **kw):
+    scale = kw.pop("scale", q.shape[2] ** -0.5)
+    lse = torch.full(q.shape[:2], float("nan"), device="cuda")
+    out = L.paged_attention(q, kp, vp, table, lens, scale=scale, lse=lse, **kw)
+    want, want_lse = attend64(q, kp, vp, table, lens, scale, kw.get("softcap", 0.0), kw.get("window", 0))
+    assert rel_l2(out, want) <= (U[q.dtype] + 1e-5 if bound is None else bound)
+    row = (out.double() - want).norm(dim=-1) / want.norm(dim=-1).clamp_min(1e-30)
+    assert float(row[lens > 0].max() if bool((lens > 0).any()) else 0) <= 2 * U[q.dtype] + 4e-5  # no single head is off
+    empty = lens <= 0
+    assert bool((out[empty] == 0).all()) and bool((lse[empty] == float("-inf")).all())
+    live = ~empty
+    assert bool(((lse[live] - want_lse[live]).abs() <= 1e-5 * (1 + want_lse[live].abs())).all())
+    return out
+
+
+EDGES = [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 0, 1000]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,page", [(32, 8, 128, 16), (8, 8, 64, 16), (20, 1, 80, 24), (4, 2, 256, 64), (16, 2, 32, 1),
+                                           (3, 3, 16, 7), (12, 1, 96, 128), (40, 1, 128, 16), (64, 2, 64, 5), (33, 1, 256, 8),
+                                           (9, 1, 8, 3)])
+def test_attention_lengths_around_every_edge(L, dtype, hq, hkv, d, page):
+    kp, vp, table, lens = cached(EDGES, hkv, d, page, dtype)
+    check_attend(L, rand(len(EDGES), hq, d, dtype=dtype, scale=1.5), kp, vp, table, lens)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[1], [4097], [100000], [30000, 1, 0, 2999], [0], [0, 0, 0]])
+def test_attention_long_and_empty(L, dtype, lens):
+    kp, vp, table, n = cached(lens, 2, 128, 16, dtype)
+    check_attend(L, rand(len(lens), 8, 128, dtype=dtype, scale=1.5), kp, vp, table, n)
+
+
+@pytest.mark.parametrize("batch", [33, 300, 1100])
+def test_attention_many_sequences(L, batch):
+    lens = [(37 * i * i + 11 * i) % 200 for i in range(batch)]
+    kp, vp, table, n = cached(lens, 2, 64, 16, torch.bfloat16)
+    check_attend(L, rand(batch, 6, 64, dtype=torch.bfloat16), kp, vp, table, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["slots", "planes"])
+@pytest.mark.parametrize("offset", [0, 1, 2])
+def test_attention_strides(L, dtype, layout, offset):
+    """Pools in other orders, q inside a projection at even and odd element offsets, a padded output."""
+    lens = [130, 5, 700]
+    kp, vp, table, n = cached(lens, 4, 64, 16, dtype, layout)
+    q = rand(3, 12 * 64 + 40, dtype=dtype)[:, offset : offset + 768].unflatten(1, (12, 64))
+    plain = L.paged_attention(q.contiguous(), kp, vp, table, n)
+    wide = torch.full((3, 12, 72), 7.0, dtype=dtype, device="cuda")
+    out = L.paged_attention(q, kp, vp, table, n, wide[..., 3:67])
+    assert torch.equal(out, plain) and bool((wide[..., :3] == 7).all()) and bool((wide[..., 67:] == 7).all())
+    check_attend(L, q, kp, vp, table, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap,window", [(30.0, 0), (0.0, 1), (0.0, 17), (5.0, 64), (0.0, 100000), (2.0, 1000)])
+def test_attention_capped_and_windowed(L, dtype, softcap, window):
+    lens = [1, 16, 17, 18, 63, 64, 65, 0, 1500, 5000]
+    kp, vp, table, n = cached(lens, 2, 64, 16, dtype)
+    check_attend(L, rand(len(lens), 8, 64, dtype=dtype, scale=4.0), kp, vp, table, n, softcap=softcap, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_extreme_scores(L, dtype):
+    """Scores far apart (one key takes all), all equal, and of the type's largest size: the running maximum keeps
+    every exponential in range."""
+    lens = [300, 64, 1025]
+    kp, vp, table, n = cached(lens, 1, 64, 16, dtype, poison=False)
+    q = rand(3, 4, 64, dtype=dtype, scale=60.0)
+    want, _ = attend64(q, kp, vp, table, n, 0.125)
+    # scores of about 60 x 8 carry 32-bit errors of about 480 x 2^-24 x 8 = 2e-4 in the exponent
+    assert rel_l2(L.paged_attention(q, kp, vp, table, n), want) <= U[dtype] + 4e-4
+    zero = torch.zeros_like(q)
+    check_attend(L, zero, kp, vp, table, n)
+    kp.fill_(1000.0)
+    q.fill_(1000.0)  # scores of 8e6: equal, so the weights are still uniform
+    got = L.paged_attention(q, kp, vp, table, n)
+    assert rel_l2(got, attend64(zero, kp, vp, table, n, 0.125)[0]) <= U[dtype] + 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_infinite_and_nan_values(L, dtype):
+    """A NaN or infinite value in a key that counts shows in its own sequence and head, and nowhere else."""
+    kp, vp, table, n = cached([100, 100, 40], 2, 64, 16, dtype)
+    clean = L.paged_attention(rand(3, 4, 64, dtype=dtype), kp, vp, table, n)
+    vp[table[0, 2], 0, 5] = float("nan")
+    kp[table[1, 1], 1, 3] = float("nan")
+    got = L.paged_attention(rand(3, 4, 64, dtype=dtype), kp, vp, table, n)
+    assert bool(got[0, :2].isnan().all()) and bool(got[1, 2:].isnan().all())
+    assert torch.equal(got[0, 2:], clean[0, 2:]) and torch.equal(got[1, :2], clean[1, :2]) and torch.equal(got[2], clean[2])
+
+
+def test_attention_lengths_and_pages_out_of_range(L):
+    """Bad page ids and lengths beyond the table are reported; the keys that exist are still used."""
+    dtype = torch.bfloat16
+    kp, vp, table, n = cached([64, 64], 2, 64, 16, dtype)
+    q = rand(2, 4, 64, dtype=dtype)
+    good = L.paged_attention(q, kp, vp, table, n)
+    # table has 5 columns, the fifth is -1
+    out = L.paged_attention(q, kp, vp, table, ints([2**31 - 1, 64]))
+    assert L.device_error() != 0
+    assert torch.equal(out[1], good[1]) and rel_l2(out[0], good[0]) <= 2 * U[dtype]
+    table[0, 1] = kp.shape[0]
+    out = L.paged_attention(q, kp, vp, table, n)
+    assert L.device_error() != 0 and torch.equal(out[1], good[1])
+    keep = table.clone()
+    keep[0] = torch.stack((table[0, 0], table[0, 2], table[0, 3], table[0, 4], table[0, 4]))
+    assert rel_l2(out[0], attend64(q, kp, vp, keep, ints([48, 64]), 0.125)[0][0]) <= U[dtype] + 1e-5
+    out = L.paged_attention(q, kp, vp, table, ints([-5, 64]))
+    assert bool((out[0] == 0).all()) and torch.equal(out[1], good[1])
+
+
+def test_attention_offsets_beyond_32_bits(L):
+    """A pool of more than 2^32 elements, the sequence's pages at its far end."""
+    dtype, hkv, page, d = torch.bfloat16, 8, 16, 128
+    n_pages = (1 << 32) // (hkv * page * d) // 2 + 200  # with keys and values together 2^32 elements
+    both = torch.empty(n_pages, 2, hkv, page, d, dtype=dtype, device="cuda")
+    assert both.numel() > 1 << 32
+    lens = [300, 1000]
+    kp, vp = both[:, 0], both[:, 1]
+    ids = torch.arange(n_pages - 90, n_pages, dtype=torch.int32, device="cuda").flip(0)
+    both[-90:] = rand(90, 2, hkv, page, d, dtype=dtype)
+    table = ids[:90].view(2, 45)
+    table = torch.cat((table, torch.full((2, 20), -1, dtype=torch.int32, device="cuda")), 1)
+    table[1] = torch.cat((ids[25:88], ids[:2]))
+    check_attend(L, rand(2, 32, d, dtype=dtype), kp, vp, table, ints(lens))
+    k, v = rand(2, hkv, d, dtype=dtype, seed=4), rand(2, hkv, d, dtype=dtype, seed=5)
+    cos, sin = tables(L, 1200, d)
+    L.rope_append(None, k, v, ints([300, 999]), cos, sin, kp, vp, table)
+    assert torch.equal(vp[table[0, 300 // 16].long(), :, 300 % 16], v[0])
+    L.page_copy(both.flatten(1, 2), ints([n_pages - 1]), ints([0]))
+    L.page_copy(both.flatten(1, 2), ints([0]), ints([n_pages - 100]))
+    assert torch.equal(both[0], both[-1]) and torch.equal(both[n_pages - 100], both[-1])
+
+
+def test_attention_repeats_bit_for_bit_and_leaves_its_workspace_ready(L):
+    kp, vp, table, n = cached([20000, 3, 900, 0, 5000], 2, 128, 16, torch.bfloat16)
+    q = rand(5, 8, 128, dtype=torch.bfloat16)
+    ws = L.paged_attention_workspace(q, kp)
+    first = L.paged_attention(q, kp, vp, table, n, workspace=ws)
+    for _ in range(20):
+        assert torch.equal(L.paged_attention(q, kp, vp, table, n, workspace=ws), first)
+    short = ints([1, 3, 900, 0, 77])  # another split of the work over the same workspace
+    a = L.paged_attention(q, kp, vp, table, short, workspace=ws)
+    assert torch.equal(a, L.paged_attention(q, kp, vp, table, short))
+    assert torch.equal(L.paged_attention(q, kp, vp, table, n, workspace=ws), first)
+
+
+def test_attention_result_does_not_depend_on_the_batch_beside_it_beyond_rounding(L):
+    kp, vp, table, n = cached([3000, 17, 5000, 250], 2, 64, 16, torch.float32)
+    q = rand(4, 8, 64)
+    whole = L.paged_attention(q, kp, vp, table, n)
+    for i in range(4):
+        assert rel_l2(L.paged_attention(q[i : i + 1], kp, vp, table[i : i + 1], n[i : i + 1]), whole[i : i + 1]) < 4e-6
+
+
+def test_attention_on_another_stream_and_in_a_graph(L):
+    kp, vp, table, n = cached([5000, 100, 1], 2, 128, 16, torch.bfloat16)
+    q = rand(3, 8, 128, dtype=torch.bfloat16)
+    want = L.paged_attention(q, kp, vp, table, n)
+    ws, out = L.paged_attention_workspace(q, kp), torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        L.paged_attention(q, kp, vp, table, n, out, workspace=ws)
+    side.synchronize()
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.paged_attention(q, kp, vp, table, n, out, workspace=ws)
+    for lens in ([5000, 100, 1], [1, 0, 1], [4999, 64, 1]):
+        n.copy_(ints(lens))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, L.paged_attention(q, kp, vp, table, n))
+
+
+# --------------------------------------------------------------- page copy
+@pytest.mark.parametrize("dtype,width", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 12), (torch.uint8, 7),
+                                         (torch.float32, 3), (torch.int64, 5)])
+@pytest.mark.parametrize("planes,page", [(1, 1), (6, 16), (512, 16), (3, 5)])
+@pytest.mark.parametrize("partial", [False, True])
+def test_page_copy(L, dtype, width, planes, page, partial):
+    n = 23
+    pages = torch.randint(0, 100, (n, planes, page, width), device="cuda").to(dtype)
+    order = torch.randperm(n)
+    src, dst = order[:9].clone(), order[9:18].clone()
+    src[3] = src[5]  # one source, two destinations
+    src[1], dst[7] = -1, -1
+    counts = torch.randint(0, page + 1, (9,)) if partial else None
+    want = pages.clone()
+    for i in range(9):
+        if src[i] >= 0 and dst[i] >= 0:
+            m = int(counts[i]) if partial else page
+            want[dst[i], :, :m] = pages[src[i], :, :m]
+    L.page_copy(pages, src.int().cuda(), dst.int().cuda(), None if counts is None else counts.int().cuda())
+    assert torch.equal(pages, want)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 4])
+def test_page_copy_views(L, offset):
+    """Planes and pages of a larger pool, at element offsets of every alignment."""
+    big = torch.randint(0, 1000, (10 * 7 * 4 * 32 + 8,), device="cuda").to(torch.float16)
+    pages = big[offset : offset + 10 * 7 * 4 * 32].view(10, 7, 4, 32)[:, 2:6]
+    want = big.clone()
+    view = want[offset : offset + 10 * 7 * 4 * 32].view(10, 7, 4, 32)[:, 2:6]
+    view[7, :, :3] = view[0, :, :3]
+    L.page_copy(pages, ints([0]), ints([7]), ints([3]))
+    assert torch.equal(big, want)
+
+
+def test_page_copy_large_and_bad_ids(L):
+    pages = torch.randint(0, 30000, (300, 64, 16, 128), device="cuda", dtype=torch.int16)
+    want = pages.clone()
+    want[150:] = pages[:150]
+    L.page_copy(pages, torch.arange(150, device="cuda", dtype=torch.int32), torch.arange(150, 300, device="cuda", dtype=torch.int32))
+    assert torch.equal(pages, want)
+    for src, dst, counts in (([300], [0], None), ([0], [2**31 - 1], None), ([0], [1], [17]), ([0], [1], [-1])):
+        L.page_copy(pages, ints(src), ints(dst), None if counts is None else ints(counts))
+        assert L.device_error() != 0 and torch.equal(pages, want)
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals(L):
+    bf, E = torch.bfloat16, L.B200KernelError
+    q, k = rand(3, 4, 64, dtype=bf), rand(3, 2, 64, dtype=bf)
+    cos, sin = tables(L, 16, 64)
+    pos = ints([0, 1, 2])
+    for bad in (lambda: L.rope(q.double(), None, pos, cos, sin), lambda: L.rope(q, k.float(), pos, cos, sin),
+                lambda: L.rope(q, k, pos.long(), cos, sin), lambda: L.rope(q, k, pos[:2], cos, sin),
+                lambda: L.rope(q, k, pos, cos.to(bf), sin.to(bf)), lambda: L.rope(q, k, pos, cos, sin[:8]),
+                lambda: L.rope(q[..., :32], None, pos, cos, sin), lambda: L.rope(q.transpose(1, 2), None, pos, cos, sin),
+                lambda: L.rope(q, k[:2], pos, cos, sin), lambda: L.rope(q, k, pos.cpu(), cos, sin),
+                lambda: L.rope(q, k, pos, cos, sin, q_out=k), lambda: L.rope(q, None, pos, cos, sin, k_out=k),
+                lambda: L.rope(q[:, 0], None, pos, cos, sin)):
+        with pytest.raises(E):
+            bad()
+    kp, vp, table, n = cached([5, 6, 7], 2, 64, 16, bf)
+    for bad in (lambda: L.rope_append(q, k, k[:, :1], pos, cos, sin, kp, vp, table),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp[:, :1], vp, table),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp.float(), vp, table),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp, vp, table[:2]),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp, vp, table.long()),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp, vp, table, seqs=pos[:2]),
+                lambda: L.rope_append(q, k, k, pos, cos, sin, kp[..., :32], vp[..., :32], table),
+                lambda: L.paged_attention(q.float(), kp, vp, table, n), lambda: L.paged_attention(q, kp, vp[:1], table, n),
+                lambda: L.paged_attention(q[:, :3], kp, vp, table, n), lambda: L.paged_attention(q, kp, vp, table[:2], n),
+                lambda: L.paged_attention(q, kp, vp, table, n[:2]), lambda: L.paged_attention(q, kp, vp, table, n.long()),
+                lambda: L.paged_attention(q, kp, vp, table, n, window=-1), lambda: L.paged_attention(q, kp, vp, table, n, softcap=-1.0),
+                lambda: L.paged_attention(q, kp, vp, table, n, softcap=float("nan")),
+                lambda: L.paged_attention(q, kp, vp, table, n, lse=torch.empty(3, 4, dtype=bf, device="cuda")),
+                lambda: L.paged_attention(q, kp, vp, table, n, workspace=torch.zeros(8, dtype=torch.uint8, device="cuda")),
+                lambda: L.paged_attention(q[..., :36].contiguous(), kp[..., :36].contiguous(), vp[..., :36].contiguous(), table, n),
+                lambda: L.paged_attention(rand(1, 1, 264, dtype=bf), rand(2, 1, 16, 264, dtype=bf), rand(2, 1, 16, 264, dtype=bf), table[:1], n[:1]),
+                lambda: L.paged_attention(q, rand(3, 2, 16, 65, dtype=bf)[..., 1:], vp, table, n),
+                lambda: L.page_copy(kp[0], pos, pos), lambda: L.page_copy(kp, pos, pos[:2]), lambda: L.page_copy(kp, pos.long(), pos),
+                lambda: L.page_copy(kp.transpose(2, 3), pos, pos), lambda: L.page_copy(kp, pos, pos.cpu())):
+        with pytest.raises(E):
+            bad()
+    empty = rand(0, 4, 64, dtype=bf)
+    assert L.paged_attention(empty, kp, vp, table[:0], n[:0]).shape == (0, 4, 64)
+    assert L.rope(empty, None, pos[:0], cos, sin)[0].shape == (0, 4, 64)
+    L.page_copy(kp, pos[:0], pos[:0])
+
+
+# -------------------------------------------------------------- all together
+def test_cache_fork_free_compact_keeps_answers(L):
+    from torch_helion.b200.kv_cache import PagedKVCache
+
+    hq, hkv, d = 8, 2, 64
+    c = PagedKVCache(2, 64, 16, hkv, d)
+    cos, sin = tables(L, 512, d)
+    a, b = c.new(), c.new()
+    step = c.extend([a, b], [75, 130])
+    for layer in range(2):
+        kv = rand(205, 2 * hkv, d, dtype=torch.bfloat16, seed=layer)
+        c.append(layer, None, kv[:, :hkv], kv[:, hkv:], cos, sin, step)
+    q = rand(1, hq, d, dtype=torch.bfloat16)
+    before = [c.attend(i, q, c.extend([b], 0)).clone() for i in range(2)]
+    kids = c.fork(b, 3)
+    c.free([a, kids[1]])
+    one = [c.attend(i, q, c.extend([kids[0]], 0)) for i in range(2)]
+    # a fork's new token goes to its own page: the others keep their answers
+    new = rand(1, 2 * hkv, d, dtype=torch.bfloat16, seed=9)
+    c.append(0, None, new[:, :hkv], new[:, hkv:], cos, sin, c.extend([kids[2]]))
+    assert c.compact() > 0
+    for seq in (b, kids[0]):
+        for i in range(2):
+            assert torch.equal(c.attend(i, q, c.extend([seq], 0)), before[i]) and torch.equal(one[i], before[i])
+    assert not torch.equal(c.attend(0, q, c.extend([kids[2]], 0)), before[0])
+
+
+def test_decoding_a_llama_stack_matches_the_blocks(L):
+    from workloads.llama_decode import main
+
+    assert main(["--layers", "2", "--hidden", "512", "--heads", "8", "--kv-heads", "2", "--intermediate", "1408",
+                 "--prompts", "1", "17", "70", "130", "--steps", "9"]) < 2e-2
+
+
+def test_odd_sizes_are_drawn(L):
+    """Random shapes over the whole range of heads, pages and lengths."""
+    import random
+
+    r = random.Random(5)
+    for i in range(24):
+        dtype = r.choice(DTYPES)
+        d = r.choice([8, 24, 40, 64, 72, 112, 128, 160, 200, 256])
+        hkv, g = r.choice([1, 2, 3, 7]), r.choice([1, 3, 4, 8, 11, 17, 30])
+        lens = [r.randint(0, int(math.exp(r.uniform(0, 8)))) for _ in range(r.randint(1, 9))]
+        kp, vp, table, n = cached(lens, hkv, d, r.randint(1, 70), dtype, r.choice(["heads", "slots", "planes"]), seed=i)
+        check_attend(L, rand(len(lens), hkv * g, d, dtype=dtype, seed=i), kp, vp, table, n,
+                     softcap=r.choice([0.0, 3.0]), window=r.choice([0, 0, r.randint(1, 300)]))

@@ -1,0 +1,206 @@
+"""Paged key-value cache without a GPU: page bookkeeping against a plain model of it, and the rotary tables.
+
+The device copy is replaced by its plain torch form, so forks and compaction
+move real data here."""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+from torch_helion.b200 import kv_cache, lib
+from torch_helion.b200.kv_cache import CacheFull, PagedKVCache, rope_tables
+
+
+def plain_page_copy(pages, src, dst, counts=None):
+    src, dst = src.tolist(), dst.tolist()
+    assert len(set(dst)) == len(dst) and not set(src) & set(dst), "destinations distinct, none a source"
+    for i, (a, b) in enumerate(zip(src, dst)):
+        n = pages.shape[2] if counts is None else int(counts[i])
+        pages[b, :, :n] = pages[a, :, :n]
+
+
+@pytest.fixture
+def cpu_cache(monkeypatch):
+    monkeypatch.setattr(kv_cache.lib, "page_copy", plain_page_copy)
+
+    def make(num_pages=24, page_size=4, **kw):
+        return PagedKVCache(2, num_pages, page_size, 1, 2, dtype=torch.float32, device="cpu", **kw)
+
+    return make
+
+
+def write(c, seqs, counts, value):
+    """Append `counts` tokens with given values the way the device append does, from the step's own tensors."""
+    step = c.extend(seqs, counts)
+    for t in range(step.positions.shape[0]):
+        pos, row = int(step.positions[t]), int(step.seqs[t])
+        page = int(step.table[row, pos // c.page_size])
+        assert page >= 0
+        c.data[page, :, :, :, pos % c.page_size] = value(seqs[row], pos)
+    return step
+
+
+def contents(c, seq):
+    n = c.length(seq)
+    return [float(c.data[c.pages(seq)[j // c.page_size], 0, 0, 0, j % c.page_size, 0]) for j in range(n)]
+
+
+def test_extend_gives_positions_rows_lengths_and_table(cpu_cache):
+    c = cpu_cache()
+    a, b = c.new(), c.new()
+    s = c.extend([a, b], [5, 0])
+    assert s.positions.tolist() == [0, 1, 2, 3, 4] and s.seqs.tolist() == [0] * 5
+    assert s.lens.tolist() == [5, 0] and s.table.tolist() == [[0, 1], [-1, -1]]
+    s = c.extend([b, a])
+    assert s.positions.tolist() == [0, 5] and s.seqs.tolist() == [0, 1] and s.lens.tolist() == [1, 6]
+    assert s.table.tolist() == [[2, -1], [0, 1]] and all(t.dtype == torch.int32 for t in (s.positions, s.seqs, s.lens, s.table))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_histories_keep_every_sequence(cpu_cache, seed):
+    """Appends, forks, frees and compactions in random order: each sequence reads back what was written to it,
+    pages are shared only when full, and none is lost."""
+    r = random.Random(seed)
+    c, want, stamp = cpu_cache(), {}, 0.0
+    for _ in range(150):
+        live, what = list(want), r.random()
+        if not live or what < 0.15:
+            want[c.new()] = []
+        elif what < 0.55:
+            seqs = r.sample(live, r.randint(1, len(live)))
+            counts = [r.randint(0, 5) for _ in seqs]
+            before = (c.free_pages, {s: c.length(s) for s in live})
+            stamp += 1000
+            try:
+                write(c, seqs, counts, lambda s, pos: stamp + 10 * s + pos)
+            except CacheFull:
+                assert before == (c.free_pages, {s: c.length(s) for s in live})
+                continue
+            for s, n in zip(seqs, counts):
+                want[s] += [stamp + 10 * s + len(want[s]) + i for i in range(n)]
+        elif what < 0.75:
+            s = r.choice(live)
+            try:
+                for child in c.fork(s, r.randint(1, 2)):
+                    want[child] = list(want[s])
+            except CacheFull:
+                pass
+        elif what < 0.9:
+            gone = r.sample(live, r.randint(1, min(2, len(live))))
+            c.free(gone)
+            for s in gone:
+                del want[s]
+        else:
+            c.compact()
+            owned = {p for s in want for p in c.pages(s)}
+            assert owned == set(range(len(owned)))
+        owned = [p for s in want for p in c.pages(s)]
+        assert len(set(owned)) + c.free_pages == c.num_pages
+        for p in set(owned):  # a shared page is full for every sequence that shares it
+            if owned.count(p) > 1:
+                assert all(c.length(s) >= (c.pages(s).index(p) + 1) * c.page_size for s in want if p in c.pages(s))
+        for s in want:
+            assert contents(c, s) == want[s]
+
+
+def test_full_pool_changes_nothing(cpu_cache):
+    c = cpu_cache(num_pages=2)
+    a = c.new()
+    c.extend([a], 7)
+    with pytest.raises(CacheFull, match="are free"):
+        c.extend([a], 2)
+    with pytest.raises(CacheFull):
+        c.fork(a)
+    assert c.length(a) == 7 and c.free_pages == 0
+    d = cpu_cache(max_pages=1)
+    with pytest.raises(CacheFull, match="allowed"):
+        d.extend([d.new()], 5)
+    assert d.free_pages == 24
+
+
+def test_refusals(cpu_cache):
+    c = cpu_cache()
+    a = c.new()
+    for seqs, counts in (([a, a], 1), ([a], [1, 2]), ([a], [-1]), ([], 1)):
+        with pytest.raises(ValueError):
+            c.extend(seqs, counts)
+    with pytest.raises(ValueError):
+        c.fork(a, 0)
+    with pytest.raises(KeyError):
+        c.free([a, a])
+    with pytest.raises(KeyError):
+        c.free(a + 1)
+    c.free(a)
+    with pytest.raises(ValueError):
+        PagedKVCache(0, 1, 1, 1, 1, device="cpu")
+
+
+# ------------------------------------------------------------ rotary tables
+def test_tables_hold_position_times_frequency():
+    cos, sin = rope_tables(40000, 64, 500000.0)
+    for pos, i in ((0, 0), (1, 0), (39999, 0), (39999, 31), (12345, 7)):
+        angle = pos * 500000.0 ** (-2 * i / 64)
+        assert abs(float(cos[pos, i]) - math.cos(angle)) < 1e-7 and abs(float(sin[pos, i]) - math.sin(angle)) < 1e-7
+
+
+def test_scaled_tables():
+    r, theta, f = 64, 10000.0, 8.0
+    plain, _ = rope_tables(4096, r, theta)
+    linear, _ = rope_tables(4096 * 8, r, theta, scaling="linear", factor=f)
+    assert torch.equal(linear[::8], plain)  # every eighth position is a plain one
+    ntk_c, ntk_s = rope_tables(64, r, theta, scaling="ntk", factor=f)
+    assert torch.equal(ntk_c[:, 0], plain[:64, 0])  # the fastest pair stays
+    slow = theta ** (-(r - 2) / r) / f
+    assert abs(float(ntk_s[50, -1]) - math.sin(50 * slow)) < 1e-7  # the slowest is slowed by the factor
+    gain = 0.1 * math.log(f) + 1
+    yc, ys = rope_tables(64, r, theta, scaling="yarn", factor=f, original=4096)
+    assert torch.allclose(yc[:, 0], plain[:64, 0] * gain, atol=1e-6)  # 652 turns in 4096 positions: kept
+    assert abs(float(ys[50, -1]) - gain * math.sin(50 * theta ** (-(r - 2) / r) / f)) < 1e-6  # 0.09 turns: slowed
+    angles = torch.atan2(ys[1], yc[1]).double()
+    full = theta ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    assert bool((angles <= full * (1 + 1e-5)).all()) and bool((angles >= full / f * (1 - 1e-5)).all())
+
+
+@pytest.mark.parametrize("kw", [{"positions": 0}, {"rotary_dim": 3}, {"scaling": "cubic"}, {"factor": 0.5},
+                                {"scaling": "yarn", "factor": 2.0}, {"scaling": "ntk", "factor": 2.0, "rotary_dim": 2}])
+def test_table_refusals(kw):
+    args = {"positions": 8, "rotary_dim": 4, **kw}
+    with pytest.raises(ValueError):
+        rope_tables(args.pop("positions"), args.pop("rotary_dim"), **args)
+
+
+# ---------------------------------------------- the binding refuses before it launches
+def test_binding_wants_cuda_tensors():
+    x = torch.zeros(2, 1, 8)
+    cos, sin = rope_tables(4, 8)
+    pos = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(lib.B200KernelError, match="CUDA"):
+        lib.rope(x, None, pos, cos, sin)
+    with pytest.raises(lib.B200KernelError, match="CUDA"):
+        lib.page_copy(torch.zeros(4, 1, 2, 8), pos, pos)
+    with pytest.raises(lib.B200KernelError, match="CUDA"):
+        lib.paged_attention(x, x[:, None], x[:, None], pos[:, None], pos)
+
+
+def test_new_argument_structs_match_the_header(tmp_path):
+    import ctypes
+    import subprocess
+
+    from conftest import REPO
+
+    names = {"th_rope_args": "RopeArgs", "th_paged_attention_args": "PagedAttentionArgs", "th_page_copy_args": "PageCopyArgs"}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{REPO / "include" / "th_b200.h"}"', "int main(void) {"]
+    for cname, pname in names.items():
+        lines.append(f'  printf("{cname} . %zu\\n", sizeof({cname}));')
+        lines += [f'  printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in getattr(lib, pname)._fields_]
+    (tmp_path / "l.c").write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.run(["gcc", "-std=c11", "-o", str(tmp_path / "l"), str(tmp_path / "l.c")], check=True)
+    out = subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout
+    for line in out.splitlines():
+        cname, field, at = line.split()
+        st = getattr(lib, names[cname])
+        assert int(at) == (ctypes.sizeof(st) if field == "." else getattr(st, field).offset), line

@@ -7,3 +7,6 @@
 #include "ssd.cu"
 #include "selftest.cu"
 #include "allreduce.cu"
+#include "rope.cu"
+#include "paged_attention.cu"
+#include "page_copy.cu"

@@ -1,0 +1,243 @@
+"""A paged key-value cache: pools of pages on the device, their bookkeeping on the host.
+
+The pool is one tensor [num_pages, layers, 2, kv_heads, page_size, head_dim],
+so a page id names the keys and values of every layer and one copy moves them
+together.  Which sequence owns which pages is plain host state (lists and
+reference counts): a scheduler has to know it without waiting for the GPU.
+Each step's row of page ids, positions and lengths goes to the device in one
+copy (:meth:`PagedKVCache.extend`).
+
+* A page is shared by the sequences forked from one another; a shared page is
+  always full, and the page that a sequence appends to is its own.
+* :meth:`PagedKVCache.compact` moves the live pages to the front of the pool.
+
+All device work runs on the current stream, in call order; use one stream per
+cache, or order the streams yourself.
+"""
+
+from __future__ import annotations
+
+import heapq
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import lib
+
+
+class CacheFull(RuntimeError):
+    """The pool has fewer free pages than the call needs; nothing was changed."""
+
+
+def rope_tables(positions: int, rotary_dim: int, theta: float = 10000.0, *, scaling: str | None = None,
+                factor: float = 1.0, original: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                device: torch.device | str = "cpu") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin of position x frequency, fp32 [positions, rotary_dim / 2], for :func:`lib.rope`.
+
+    Frequencies are theta ** (-2 i / rotary_dim); angles are formed in 64 bits and rounded once as
+    cos and sin, so a long context loses nothing.  ``scaling`` stretches them for contexts ``factor``
+    times longer:
+
+    * ``"linear"``: every position counts 1 / factor;
+    * ``"ntk"``: the base becomes theta * factor ** (r / (r - 2)), which leaves the fastest pair as it
+      is and slows the slowest by factor;
+    * ``"yarn"``: pairs that turn more than ``beta_fast`` times within ``original`` positions keep
+      their frequency, those below ``beta_slow`` turns are slowed by factor, the ones between are
+      blended linearly in the pair index, and cos and sin carry the factor 0.1 ln(factor) + 1."""
+    if positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rope_tables: needs at least one position and an even rotary_dim")
+    if factor < 1.0 or (scaling == "ntk" and rotary_dim < 4) or (scaling == "yarn" and original < 1):
+        raise ValueError("rope_tables: factor must be at least 1, ntk needs rotary_dim >= 4, yarn the original length")
+    exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    gain = 1.0
+    if scaling == "ntk":
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = theta ** -exponent
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        # index of the pair that turns `turns` times in `original` positions
+        def index(turns: float) -> float:
+            return rotary_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta))
+
+        low = max(0.0, math.floor(index(beta_fast)))
+        high = min(rotary_dim / 2 - 1, math.ceil(index(beta_slow)))
+        blend = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq * (1 - blend) + freq / factor * blend
+        gain = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rope_tables: unknown scaling {scaling!r} (linear, ntk, yarn)")
+    freq = freq.to(device)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return (angle.cos() * gain).float(), (angle.sin() * gain).float()
+
+
+@dataclass
+class Step:
+    """Device inputs of one step over a batch of sequences (all int32)."""
+
+    positions: torch.Tensor  # [tokens] position of every new token
+    seqs: torch.Tensor       # [tokens] its row of ``table``
+    lens: torch.Tensor       # [batch] length of each sequence with the new tokens
+    table: torch.Tensor      # [batch, columns] page ids, -1 where there is none
+
+
+class PagedKVCache:
+    """See the module's text.  ``max_pages`` bounds the pages of one sequence (None: the pool)."""
+
+    def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, *,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
+                 max_pages: int | None = None) -> None:
+        if min(layers, num_pages, page_size, kv_heads, head_dim) < 1:
+            raise ValueError("PagedKVCache: every size must be at least 1")
+        self.layers, self.num_pages, self.page_size = layers, num_pages, page_size
+        self.max_pages = max_pages
+        self.device = torch.device(device)
+        self.data = torch.empty(num_pages, layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=self.device)
+        self._refs = [0] * num_pages
+        self._free = list(range(num_pages))  # a heap: the lowest free id first keeps the pool's front dense
+        self._pages: dict[int, list[int]] = {}
+        self._len: dict[int, int] = {}
+        self._next = 0
+        self._workspace: dict[int, torch.Tensor] = {}
+
+    # ------------------------------------------------------------ bookkeeping
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._len[seq]
+
+    def pages(self, seq: int) -> list[int]:
+        """The page ids of a sequence, in order."""
+        return list(self._pages[seq])
+
+    def new(self) -> int:
+        """An empty sequence."""
+        seq = self._next
+        self._next += 1
+        self._pages[seq], self._len[seq] = [], 0
+        return seq
+
+    def _take(self) -> int:
+        page = heapq.heappop(self._free)
+        self._refs[page] = 1
+        return page
+
+    def extend(self, seqs: list[int], counts: list[int] | int = 1) -> Step:
+        """Room for ``counts`` more tokens of each sequence, and the step's device inputs.
+
+        The tokens are those of ``seqs[0]``, then ``seqs[1]``, and so on.  Raises :class:`CacheFull`
+        without any change when the pool has too few pages."""
+        if isinstance(counts, int):
+            counts = [counts] * len(seqs)
+        if len(counts) != len(seqs) or len(set(seqs)) != len(seqs) or min(counts, default=0) < 0 or not seqs:
+            raise ValueError("extend: one count (>= 0) for each of at least one distinct sequence")
+        ps = self.page_size
+        need = [-(-(self._len[s] + n) // ps) for s, n in zip(seqs, counts)]
+        if self.max_pages is not None and max(need) > self.max_pages:
+            raise CacheFull(f"a sequence needs {max(need)} pages, {self.max_pages} are allowed")
+        more = sum(n - len(self._pages[s]) for s, n in zip(seqs, need))
+        if more > len(self._free):
+            raise CacheFull(f"{more} pages are needed, {len(self._free)} are free")
+        positions: list[int] = []
+        rows: list[int] = []
+        for r, (s, n, k) in enumerate(zip(seqs, need, counts)):
+            self._pages[s] += [self._take() for _ in range(n - len(self._pages[s]))]
+            positions += range(self._len[s], self._len[s] + k)
+            rows += [r] * k
+            self._len[s] += k
+        cols = max(1, max(need))
+        table = torch.full((len(seqs), cols), -1, dtype=torch.int32)
+        for r, s in enumerate(seqs):
+            table[r, : len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
+        lens = torch.tensor([self._len[s] for s in seqs], dtype=torch.int32)
+        # one buffer, one copy; torch's pinned allocator keeps the staging memory until the copy has run
+        host = torch.cat((torch.tensor(positions, dtype=torch.int32), torch.tensor(rows, dtype=torch.int32), lens,
+                          table.reshape(-1)))
+        if self.device.type == "cuda":
+            dev = host.pin_memory().to(self.device, non_blocking=True)
+        else:
+            dev = host
+        a, b = len(positions), len(seqs)
+        return Step(dev[:a], dev[a : 2 * a], dev[2 * a : 2 * a + b], dev[2 * a + b :].view(b, cols))
+
+    def fork(self, seq: int, n: int = 1) -> list[int]:
+        """``n`` new sequences with the contents of ``seq``: full pages are shared, the last, partly
+        filled one is copied for each."""
+        if n < 1:
+            raise ValueError("fork: at least one copy")
+        pages, used = self._pages[seq], self._len[seq] % self.page_size
+        full = self._len[seq] // self.page_size
+        if used and n > len(self._free):
+            raise CacheFull(f"{n} pages are needed, {len(self._free)} are free")
+        out, src, dst = [], [], []
+        for _ in range(n):
+            child = self.new()
+            self._pages[child] = pages[:full]
+            for page in pages[:full]:
+                self._refs[page] += 1
+            if used:
+                self._pages[child].append(self._take())
+                src.append(pages[full])
+                dst.append(self._pages[child][-1])
+            self._len[child] = self._len[seq]
+            out.append(child)
+        self._copy(src, dst, [used] * len(src))
+        return out
+
+    def free(self, seqs: list[int] | int) -> None:
+        """Drop sequences; pages that no other sequence shares return to the pool."""
+        seqs = [seqs] if isinstance(seqs, int) else list(seqs)
+        missing = [s for s in seqs if s not in self._pages]
+        if missing or len(set(seqs)) != len(seqs):
+            raise KeyError(f"free: unknown or repeated sequences {missing or seqs}")
+        for s in seqs:
+            for page in self._pages.pop(s):
+                self._refs[page] -= 1
+                if self._refs[page] == 0:
+                    heapq.heappush(self._free, page)
+            del self._len[s]
+
+    def compact(self) -> int:
+        """Move live pages into the lowest ids; returns how many moved.  Steps made before are void.
+
+        Only pages at or beyond the live count move, into the holes below it, so no page is both
+        read and written."""
+        live = self.num_pages - len(self._free)
+        holes = sorted(p for p in self._free if p < live)
+        late = [p for p in range(live, self.num_pages) if self._refs[p]]
+        moved = dict(zip(late, holes))
+        self._copy(late, holes, None)
+        for src, dst in moved.items():
+            self._refs[dst], self._refs[src] = self._refs[src], 0
+        for s, pages in self._pages.items():
+            self._pages[s] = [moved.get(p, p) for p in pages]
+        self._free = list(range(live, self.num_pages))
+        return len(moved)
+
+    def _copy(self, src: list[int], dst: list[int], counts: list[int] | None) -> None:
+        if not src:
+            return
+        host = torch.tensor([src, dst] + ([counts] if counts else []), dtype=torch.int32)
+        ids = host.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else host
+        lib.page_copy(self.data.flatten(1, 3), ids[0], ids[1], ids[2] if counts else None)
+
+    # ------------------------------------------------------------ device work
+    def layer(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) of layer ``i``: views [num_pages, kv_heads, page_size, head_dim]."""
+        return self.data[:, i, 0], self.data[:, i, 1]
+
+    def append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+               sin: torch.Tensor, step: Step, **kw) -> torch.Tensor | None:
+        """Rotate q and k and store the step's keys and values (:func:`lib.rope_append`)."""
+        return lib.rope_append(q, k, v, step.positions, cos, sin, *self.layer(layer), step.table, seqs=step.seqs, **kw)
+
+    def attend(self, layer: int, q: torch.Tensor, step: Step, **kw) -> torch.Tensor:
+        """Attention of one new token per sequence (:func:`lib.paged_attention`)."""
+        keys, values = self.layer(layer)
+        if q.shape[1] not in self._workspace:
+            self._workspace[q.shape[1]] = lib.paged_attention_workspace(q, keys)
+        return lib.paged_attention(q, keys, values, step.table, step.lens, workspace=self._workspace[q.shape[1]], **kw)

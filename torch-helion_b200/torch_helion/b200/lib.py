@@ -28,7 +28,8 @@ _DTYPES = {torch.float32: TH_F32, torch.bfloat16: TH_BF16, torch.float16: TH_F16
 EXPORTED_SYMBOLS = (
     "th_last_error_string", "th_version", "th_device_error", "th_rowstat", "th_rmsnorm", "th_gemm",
     "th_attention", "th_conv1d", "th_ssd_workspace_size", "th_ssd", "th_embedding", "th_ssd_noalloc",
-    "th_selftest_bounded_wait", "th_allreduce",
+    "th_selftest_bounded_wait", "th_allreduce", "th_rope", "th_rope_append", "th_paged_attention_workspace_size",
+    "th_paged_attention", "th_page_copy",
 )
 
 
@@ -97,6 +98,38 @@ class EmbeddingArgs(ctypes.Structure):
                 ("dim", _i64), ("vocab", _i64), ("dtype", _i32)]
 
 
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_token", _i64), ("q_head", _i64), ("q_out", _vp), ("qo_token", _i64), ("qo_head", _i64),
+        ("k", _vp), ("k_token", _i64), ("k_head", _i64), ("k_out", _vp), ("ko_token", _i64), ("ko_head", _i64),
+        ("positions", _vp), ("cos", _vp), ("sin", _vp), ("ld_cs", _i64), ("tokens", _i64),
+        ("table_rows", _i32), ("hq", _i32), ("hkv", _i32), ("head_dim", _i32), ("rotary_dim", _i32),
+        ("interleaved", _i32), ("inverse", _i32), ("dtype", _i32),
+        ("v", _vp), ("v_token", _i64), ("v_head", _i64), ("k_pages", _vp), ("k_page", _i64), ("k_phead", _i64),
+        ("k_slot", _i64), ("v_pages", _vp), ("v_page", _i64), ("v_phead", _i64), ("v_slot", _i64),
+        ("table", _vp), ("ld_table", _i64), ("seqs", _vp),
+        ("batch", _i32), ("table_cols", _i32), ("page_size", _i32), ("num_pages", _i32),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_row", _i64), ("q_head", _i64), ("o", _vp), ("o_row", _i64), ("o_head", _i64), ("lse", _vp),
+        ("k_pages", _vp), ("k_page", _i64), ("k_head", _i64), ("k_slot", _i64),
+        ("v_pages", _vp), ("v_page", _i64), ("v_head", _i64), ("v_slot", _i64),
+        ("table", _vp), ("ld_table", _i64), ("lens", _vp),
+        ("batch", _i32), ("hq", _i32), ("hkv", _i32), ("head_dim", _i32), ("page_size", _i32), ("num_pages", _i32),
+        ("table_cols", _i32), ("window", _i32), ("scale", _f32), ("softcap", _f32), ("dtype", _i32),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PageCopyArgs(ctypes.Structure):
+    _fields_ = [("pages", _vp), ("page_stride", _i64), ("plane_stride", _i64), ("slot_bytes", _i64), ("src", _vp),
+                ("dst", _vp), ("counts", _vp), ("pairs", _i32), ("num_pages", _i32), ("planes", _i32),
+                ("page_size", _i32)]
+
+
 _LIB: ctypes.CDLL | None = None
 
 
@@ -133,10 +166,13 @@ def load() -> ctypes.CDLL:
         for name, st in (("th_rowstat", RowstatArgs), ("th_rmsnorm", RmsnormArgs), ("th_gemm", GemmArgs),
                          ("th_attention", AttentionArgs), ("th_conv1d", Conv1dArgs), ("th_ssd", SsdArgs),
                          ("th_ssd_noalloc", SsdArgs), ("th_embedding", EmbeddingArgs),
-                         ("th_allreduce", AllreduceArgs)):
+                         ("th_allreduce", AllreduceArgs), ("th_rope", RopeArgs), ("th_rope_append", RopeArgs),
+                         ("th_paged_attention", PagedAttentionArgs), ("th_page_copy", PageCopyArgs)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(st), _vp]
+        lib.th_paged_attention_workspace_size.restype = ctypes.c_size_t
+        lib.th_paged_attention_workspace_size.argtypes = [_i32] * 4
         lib.th_device_error.restype = ctypes.c_int
         lib.th_device_error.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.c_int]
         lib.th_selftest_bounded_wait.restype = ctypes.c_int
@@ -360,3 +396,225 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torc
                       _dt(table))
     _check(load().th_embedding(ctypes.byref(a), _stream()), "th_embedding")
     return out
+
+
+# ------------------------------------------------------- cached decoding
+def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
+    """(token stride, head stride) of a [tokens, heads, head_dim] view with unit element stride."""
+    st = t.stride()
+    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
+        raise B200KernelError(f"{what} must be [tokens, heads, head_dim] with unit element stride, got shape "
+                              f"{tuple(t.shape)} stride {st}")
+    return st[0], st[1]
+
+
+def _pool(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(page, head, slot) strides of a page pool [num_pages, heads, page_size, head_dim]."""
+    st = t.stride()
+    if len(st) != 4 or st[3] != 1:
+        raise B200KernelError(f"{what} must be [num_pages, heads, page_size, head_dim] with unit element stride, got "
+                              f"shape {tuple(t.shape)} stride {st}")
+    return st[0], st[1], st[2]
+
+
+def _ints(t: torch.Tensor, n: int, what: str) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise B200KernelError(f"{what} must be contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _page_table(table: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(rows, columns, leading dimension) of an int32 page table."""
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise B200KernelError(f"{what} must be int32 [sequences, columns] with unit column stride, got {table.dtype} "
+                              f"{tuple(table.shape)}")
+    return table.shape[0], table.shape[1], table.stride(0)
+
+
+def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    dev = first.device
+    if dev.type != "cuda":
+        raise B200KernelError("all tensors must live on a CUDA device")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise B200KernelError(f"all tensors must live on {dev}, got one on {t.device}")
+
+
+def _rope_args(what: str, x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+               interleaved: bool) -> RopeArgs:
+    a = RopeArgs()
+    tokens, _, d = x.shape
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
+            or cos.stride() != sin.stride() or (cos.shape[1] > 1 and cos.stride(1) != 1)):
+        raise B200KernelError(f"{what}: cos and sin must be fp32 [positions, rotary_dim / 2] of one layout")
+    rotary = 2 * cos.shape[1]
+    if rotary > d:
+        raise B200KernelError(f"{what}: the tables rotate {rotary} elements of heads of {d}")
+    a.positions = _ints(positions, tokens, f"{what}: positions")
+    a.cos, a.sin, a.ld_cs, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
+    a.tokens, a.head_dim, a.rotary_dim, a.interleaved, a.dtype = tokens, d, rotary, int(interleaved), _dt(x)
+    return a
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
+         q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, interleaved: bool = False,
+         inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions on ``q`` [tokens, hq, d] and ``k`` [tokens, hkv, d] (or None) in one launch.
+
+    ``positions`` int32 [tokens] are rows of the fp32 tables ``cos``, ``sin`` [positions, rotary_dim / 2]
+    (:func:`torch_helion.b200.kv_cache.rope_tables`); a rotary_dim below d leaves the rest of each head
+    as it is.  Pairs are (i, i + rotary_dim / 2), or with ``interleaved`` (2i, 2i + 1).  ``inverse``
+    turns back: the gradient with respect to the input is ``rope(grad, ..., inverse=True)``.  An output
+    may be its input.  A negative position marks padding (zeros); one beyond the tables sets the device
+    error word.  Returns ``(q_out, k_out)``."""
+    _same_device(q, k, positions, cos, sin, q_out, k_out)
+    q_tok, q_head = _heads(q, "rope: q")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+        raise B200KernelError("rope: q_out must have q's shape and dtype")
+    a = _rope_args("rope", q, positions, cos, sin, interleaved)
+    a.q, a.q_token, a.q_head, a.hq = q.data_ptr(), q_tok, q_head, q.shape[1]
+    a.q_out, (a.qo_token, a.qo_head) = q_out.data_ptr(), _heads(q_out, "rope: q_out")
+    if k is not None:
+        if k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise B200KernelError("rope: k must be [tokens, heads, head_dim] like q, of q's dtype")
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        elif k_out.shape != k.shape or k_out.dtype != k.dtype:
+            raise B200KernelError("rope: k_out must have k's shape and dtype")
+        a.k, (a.k_token, a.k_head), a.hkv = k.data_ptr(), _heads(k, "rope: k"), k.shape[1]
+        a.k_out, (a.ko_token, a.ko_head) = k_out.data_ptr(), _heads(k_out, "rope: k_out")
+    elif k_out is not None:
+        raise B200KernelError("rope: k_out without k")
+    a.inverse = int(inverse)
+    if a.tokens:
+        _check(load().th_rope(ctypes.byref(a), _stream()), "th_rope")
+    return q_out, k_out
+
+
+def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
+                sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, *,
+                seqs: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                k_out: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+    """Rotate ``q`` and ``k`` and store rotated keys and values in a paged cache, in one launch.
+
+    Token t belongs to sequence ``seqs[t]`` (int32; None: sequence t) at ``positions[t]``; its key and
+    value go to slot ``position % page_size`` of page ``table[sequence, position // page_size]`` of the
+    pools [num_pages, hkv, page_size, d] (any page, head and slot strides).  A negative position marks
+    padding: nothing is stored and its q_out row is zero.  Ids out of range set the device error word.
+    ``k_out`` (optional, like k) receives the rotated keys as well.  Returns ``q_out`` (None without q)."""
+    _same_device(k, q, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out)
+    a = _rope_args("rope_append", k, positions, cos, sin, interleaved)
+    tokens, hkv, d = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise B200KernelError("rope_append: v must have k's shape and dtype")
+    for pool in (k_pages, v_pages):
+        if pool.dtype != k.dtype or pool.dim() != 4 or pool.shape != k_pages.shape or pool.shape[1] != hkv or pool.shape[3] != d:
+            raise B200KernelError("rope_append: the pools must be [num_pages, hkv, page_size, d] of k's dtype")
+    if q is not None:
+        if q.dtype != k.dtype or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != d:
+            raise B200KernelError("rope_append: q must be [tokens, heads, head_dim] like k, of k's dtype")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise B200KernelError("rope_append: q_out must have q's shape and dtype")
+        a.q, (a.q_token, a.q_head), a.hq = q.data_ptr(), _heads(q, "rope_append: q"), q.shape[1]
+        a.q_out, (a.qo_token, a.qo_head) = q_out.data_ptr(), _heads(q_out, "rope_append: q_out")
+    elif q_out is not None:
+        raise B200KernelError("rope_append: q_out without q")
+    a.k, (a.k_token, a.k_head), a.hkv = k.data_ptr(), _heads(k, "rope_append: k"), hkv
+    if k_out is not None:
+        if k_out.shape != k.shape or k_out.dtype != k.dtype:
+            raise B200KernelError("rope_append: k_out must have k's shape and dtype")
+        a.k_out, (a.ko_token, a.ko_head) = k_out.data_ptr(), _heads(k_out, "rope_append: k_out")
+    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, "rope_append: v")
+    a.k_pages, (a.k_page, a.k_phead, a.k_slot) = k_pages.data_ptr(), _pool(k_pages, "rope_append: k_pages")
+    a.v_pages, (a.v_page, a.v_phead, a.v_slot) = v_pages.data_ptr(), _pool(v_pages, "rope_append: v_pages")
+    a.table, (a.batch, a.table_cols, a.ld_table) = table.data_ptr(), _page_table(table, "rope_append: table")
+    a.num_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
+    if seqs is not None:
+        a.seqs = _ints(seqs, tokens, "rope_append: seqs")
+    elif a.batch < tokens:
+        raise B200KernelError(f"rope_append: {tokens} tokens without seqs need as many rows of table, got {a.batch}")
+    if tokens:
+        _check(load().th_rope_append(ctypes.byref(a), _stream()), "th_rope_append")
+    return q_out
+
+
+def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor) -> torch.Tensor:
+    """A zeroed workspace for :func:`paged_attention` calls with heads like these (any batch, any lengths)."""
+    need = load().th_paged_attention_workspace_size(q.shape[1], k_pages.shape[1], q.shape[2], _dt(q))
+    if need == 0:
+        raise B200KernelError(f"paged_attention: heads {q.shape[1]} over {k_pages.shape[1]} of {q.shape[2]} are not supported")
+    return torch.zeros(int(need), dtype=torch.uint8, device=q.device)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                    lens: torch.Tensor, out: torch.Tensor | None = None, *, scale: float | None = None,
+                    softcap: float = 0.0, window: int = 0, lse: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over the paged cache.
+
+    ``q`` [batch, hq, d]; pools [num_pages, hkv, page_size, d] (any page, head and slot strides);
+    ``table`` int32 [batch, columns]; ``lens`` int32 [batch], the keys of each sequence with the new
+    token's own (0: the output row is zero).  ``scale`` defaults to d ** -0.5; ``softcap`` > 0 caps the
+    scores as softcap * tanh(score / softcap); ``window`` > 0 keeps the last ``window`` keys.  ``lse``
+    (fp32 [batch, hq], optional) receives log sum exp of the scores.  ``workspace`` comes from
+    :func:`paged_attention_workspace` and may be kept; calls that share one must be ordered on the GPU
+    (None: a fresh one per call)."""
+    _same_device(q, k_pages, v_pages, table, lens, out, lse, workspace)
+    q_row, q_head = _heads(q, "paged_attention: q")
+    batch, hq, d = q.shape
+    pool = _pool(k_pages, "paged_attention: k_pages")
+    num_pages, hkv, page_size, dk = k_pages.shape
+    if v_pages.shape != k_pages.shape or dk != d or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise B200KernelError("paged_attention: the pools must be [num_pages, hkv, page_size, d] of q's dtype and head size")
+    rows, cols, ld = _page_table(table, "paged_attention: table")
+    if rows < batch:
+        raise B200KernelError(f"paged_attention: {batch} queries need as many rows of table, got {rows}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise B200KernelError("paged_attention: out must have q's shape and dtype")
+    if batch == 0:
+        return out
+    if workspace is None:
+        workspace = paged_attention_workspace(q, k_pages)
+    a = PagedAttentionArgs()
+    a.q, a.q_row, a.q_head = q.data_ptr(), q_row, q_head
+    a.o, (a.o_row, a.o_head) = out.data_ptr(), _heads(out, "paged_attention: out")
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous():
+            raise B200KernelError("paged_attention: lse must be contiguous fp32 [batch, hq]")
+        a.lse = lse.data_ptr()
+    a.k_pages, (a.k_page, a.k_head, a.k_slot) = k_pages.data_ptr(), pool
+    a.v_pages, (a.v_page, a.v_head, a.v_slot) = v_pages.data_ptr(), _pool(v_pages, "paged_attention: v_pages")
+    a.table, a.ld_table, a.lens = table.data_ptr(), ld, _ints(lens, batch, "paged_attention: lens")
+    a.batch, a.hq, a.hkv, a.head_dim, a.page_size, a.num_pages, a.table_cols = batch, hq, hkv, d, page_size, num_pages, cols
+    a.window, a.softcap, a.dtype = window, softcap, _dt(q)
+    a.scale = d ** -0.5 if scale is None else scale
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _check(load().th_paged_attention(ctypes.byref(a), _stream()), "th_paged_attention")
+    return out
+
+
+def page_copy(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+    """Copy pages of a pool in place: ``pages[dst[i], :, :counts[i]] = pages[src[i], :, :counts[i]]``.
+
+    ``pages`` [num_pages, planes, page_size, width] of any dtype (slots contiguous; planes are every
+    plane that shares the page ids: layers x keys and values x heads), ``src``, ``dst`` and ``counts``
+    int32 [pairs] (counts None: whole pages).  A negative id skips the pair.  Destinations must be
+    distinct and none may be a source; ids out of range set the device error word."""
+    _same_device(pages, src, dst, counts)
+    if pages.dim() != 4 or pages.stride(3) != 1 or (pages.shape[2] > 1 and pages.stride(2) != pages.shape[3]):
+        raise B200KernelError("page_copy: pages must be [num_pages, planes, page_size, width] with contiguous slots, got "
+                              f"shape {tuple(pages.shape)} stride {pages.stride()}")
+    n, es = src.shape[0] if src.dim() == 1 else -1, pages.element_size()
+    if n == 0 or pages.numel() == 0:
+        return
+    a = PageCopyArgs(pages.data_ptr(), pages.stride(0) * es, pages.stride(1) * es, pages.shape[3] * es,
+                     _ints(src, n, "page_copy: src"), _ints(dst, n, "page_copy: dst"),
+                     None if counts is None else _ints(counts, n, "page_copy: counts"), n, pages.shape[0],
+                     pages.shape[1], pages.shape[2])
+    _check(load().th_page_copy(ctypes.byref(a), _stream()), "th_page_copy")

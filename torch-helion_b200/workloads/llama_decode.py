@@ -1,0 +1,152 @@
+"""Token-by-token answers of a stack of Llama blocks over a paged key-value cache.
+
+    python -m workloads.llama_decode --layers 2 --steps 16        (from torch-helion_b200/)
+
+Runs prompts of different lengths into the cache, answers them one token at a
+time as a batch, forks one of the sequences, drops another and compacts the
+pool, and checks every sequence's last state against the blocks run over that
+whole sequence at once.
+"""
+
+from __future__ import annotations
+
+import argparse
+import time
+from dataclasses import dataclass
+
+import torch
+
+from torch_helion.b200 import lib
+from torch_helion.b200.kv_cache import PagedKVCache, Step, rope_tables
+from torch_helion.optimizer.param_transforms import swiglu_interleave
+
+from .llama_block import LlamaBlock, LlamaBlockConfig, build_llama_block
+
+
+@dataclass
+class _Layer:
+    qkv: torch.Tensor      # [(hq + 2 hkv) d, hidden], the input norm's gain folded in
+    o: torch.Tensor
+    gate_up: torch.Tensor  # gate and up in alternating blocks of 64 rows, the post norm's gain folded in
+    down: torch.Tensor
+
+
+class LlamaDecoder:
+    """Serves ``blocks`` (same configuration, causal) from a cache of ``num_pages`` pages."""
+
+    def __init__(self, blocks: list[LlamaBlock], num_pages: int, page_size: int = 16, positions: int = 8192,
+                 device: torch.device | str = "cuda") -> None:
+        c = self.cfg = blocks[0].cfg
+        if not c.causal or any(b.cfg != c for b in blocks):
+            raise ValueError("LlamaDecoder: causal blocks of one configuration")
+        self.layers = []
+        for b in blocks:
+            def w(*ws, gain=None):
+                m = torch.cat([x.detach().float() for x in ws])
+                return (m if gain is None else m * gain.detach().float()).to(device=device, dtype=c.dtype)
+
+            a, m = b.attn, b.mlp
+            gate_up = swiglu_interleave(m.gate_proj.weight.detach().float(), m.up_proj.weight.detach().float())
+            self.layers.append(_Layer(w(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, gain=b.input_norm.weight),
+                                      w(a.o_proj.weight), w(gate_up, gain=b.post_norm.weight), w(m.down_proj.weight)))
+        self.cos, self.sin = rope_tables(positions, c.head_dim, c.rope_theta, device=device)
+        self.cache = PagedKVCache(len(blocks), num_pages, page_size, c.n_kv, c.head_dim, dtype=c.dtype, device=device)
+
+    def _norm(self, x: torch.Tensor) -> dict:
+        return {"rs_parts": lib.rowstat(x).reshape(-1, 1), "rs_inv_k": 1.0 / self.cfg.hidden, "rs_eps": self.cfg.eps}
+
+    def _forward(self, x: torch.Tensor, step: Step, prompts: list[int] | None) -> torch.Tensor:
+        c, new = self.cfg, lambda n: torch.empty(x.shape[0], n, dtype=x.dtype, device=x.device)
+        hq, hkv, d = c.heads, c.n_kv, c.head_dim
+        for i, w in enumerate(self.layers):
+            qkv = lib.gemm(x, w.qkv, new((hq + 2 * hkv) * d), **self._norm(x)).view(-1, hq + 2 * hkv, d)
+            q, k, v = qkv[:, :hq], qkv[:, hq : hq + hkv], qkv[:, hq + hkv :]
+            turned = torch.empty_like(k) if prompts else None
+            q = self.cache.append(i, q, k, v, self.cos, self.sin, step, k_out=turned)
+            if prompts:
+                a, t = new(hq * d), 0
+                for n in prompts:
+                    part = slice(t, t + n)
+                    lib.attention(q[part].view(n, -1), turned[part].view(n, -1), qkv.view(x.shape[0], -1)[part, (hq + hkv) * d :],
+                                  a[part], batch=1, seq=n, hq=hq, hkv=hkv, head_dim=d, scale=d ** -0.5, causal=True)
+                    t += n
+            else:
+                a = self.cache.attend(i, q, step).view(-1, hq * d)
+            h = lib.gemm(a, w.o, new(c.hidden), residual=x)
+            f = lib.gemm(h, w.gate_up, new(c.intermediate), swiglu=True, **self._norm(h))
+            x = lib.gemm(f, w.down, new(c.hidden), residual=h)
+        return x
+
+    def prompt(self, xs: list[torch.Tensor]) -> tuple[list[int], torch.Tensor]:
+        """New sequences from prompts [length, hidden] each: their ids and the stacked outputs [sum of lengths, hidden]."""
+        seqs, lens = [self.cache.new() for _ in xs], [x.shape[0] for x in xs]
+        step = self.cache.extend(seqs, lens)
+        return seqs, self._forward(torch.cat(xs), step, lens)
+
+    def step(self, seqs: list[int], x: torch.Tensor) -> torch.Tensor:
+        """One new token [len(seqs), hidden] for each sequence."""
+        return self._forward(x, self.cache.extend(seqs, 1), None)
+
+
+def main(argv: list[str] | None = None) -> float:
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--layers", type=int, default=2)
+    ap.add_argument("--hidden", type=int, default=1024)
+    ap.add_argument("--heads", type=int, default=8)
+    ap.add_argument("--kv-heads", type=int, default=2)
+    ap.add_argument("--intermediate", type=int, default=2816)
+    ap.add_argument("--prompts", type=int, nargs="+", default=[1, 17, 100, 333])
+    ap.add_argument("--steps", type=int, default=16)
+    a = ap.parse_args(argv)
+    longest = max(a.prompts) + a.steps
+    cfg = LlamaBlockConfig(batch=1, seq=longest, hidden=a.hidden, heads=a.heads, intermediate=a.intermediate,
+                           dtype=torch.bfloat16, kv_heads=a.kv_heads, causal=True)
+    blocks = [build_llama_block(cfg, seed) for seed in range(a.layers)]
+    page = 16
+    dec = LlamaDecoder(blocks, sum(-(-(n + a.steps) // page) for n in a.prompts) + 2 * -(-longest // page), page, longest)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, a.hidden, generator=gen, device="cuda").to(cfg.dtype)
+    xs = [rand(n) for n in a.prompts]
+    seqs, _ = dec.prompt(xs)
+    seen = {s: [x] for s, x in zip(seqs, xs)}
+    half = a.steps // 2
+    last: dict[int, torch.Tensor] = {}
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    for i in range(a.steps):
+        if i == half:  # one more answer to the longest prompt, one sequence less, the pool compacted
+            parent = seqs[max(range(len(seqs)), key=lambda j: dec.cache.length(seqs[j]))]
+            child = dec.cache.fork(parent)[0]
+            seen[child] = list(seen[parent])
+            gone = seqs[0]
+            dec.cache.free(gone)
+            dec.cache.compact()
+            seqs = seqs[1:] + [child]
+        x = rand(len(seqs))
+        y = dec.step(seqs, x)
+        for j, s in enumerate(seqs):
+            seen[s].append(x[j : j + 1])
+            last[s] = y[j]
+    torch.cuda.synchronize()
+    dt = time.perf_counter() - t0
+    if lib.device_error():
+        raise RuntimeError("a kernel reported an error")
+    worst = 0.0
+    for s in seqs:
+        h = torch.cat(seen[s]).float().cpu()[None]
+        for b in blocks:
+            n = h.shape[1]
+            fb = build_llama_block(LlamaBlockConfig(**{**cfg.__dict__, "seq": n, "dtype": torch.float32}))
+            fb.load_state_dict({k: v.float() if k in dict(b.named_parameters()) else dict(fb.named_buffers())[k]
+                                for k, v in b.state_dict().items()})
+            h = fb(h).detach()
+        ref = h[0, -1]
+        worst = max(worst, float((last[s].float().cpu() - ref).norm() / ref.norm()))
+    print(f"{a.layers} layers, {len(seqs)} sequences of {min(map(dec.cache.length, seqs))} to "
+          f"{max(map(dec.cache.length, seqs))} tokens: {1e3 * dt / a.steps:.2f} ms a step, last states within {worst:.1e} "
+          "of the blocks in fp32")
+    return worst
+
+
+if __name__ == "__main__":
+    main()
