@@ -1,86 +1,723 @@
 // th_paged_attention: attention of one new token per sequence over a paged
 // key-value cache.
+//
+// Every key and value is read once, so the floor is their bytes at the copy
+// rate; the arithmetic (4 flops per cached element and query head) is far
+// below it.  The kernel therefore is a stream of cp.async copies with a little
+// work behind it:
+//
+// * Work is cut into tiles of 4 KB keys (KB per warp) of one (sequence, key-
+//   value head, block of query heads), numbered in that order over the whole
+//   batch.  Every CTA takes an equal run of tiles, so ragged lengths, one long
+//   sequence or a thousand short ones load the SMs alike, and nothing about
+//   the lengths has to be known on the host (a captured graph stays valid).
+// * Each warp keeps its own ring of S blocks of KB keys and values and its own
+//   running maximum, sum and accumulator: no block-wide wait inside a run.
+// * A CTA that ends a (sequence, head) joins its four warps; where a run cuts
+//   the item, every CTA on it leaves a partial result, and the one that comes
+//   last (an atomic count) adds them up in a fixed order, so the result does
+//   not depend on which CTA that is.
 #include "common.cuh"
 
 namespace th {
 
-// One block per (sequence, query head).  Each warp takes every fourth key:
-// lanes hold the head's elements, the running maximum and sum are per warp
-// and the four warps join at the end.
+constexpr int PA_WARPS = 4;
+constexpr float PA_LOG2E = 1.4426950408889634f;
+constexpr float PA_LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// Transpose of an 8x8 matrix of 16-bit elements held in fragment order.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 template <typename T>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const __grid_constant__ th_paged_attention_args p) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float4 lds128(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 lds64(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// What the host adds to the arguments.
+struct PaPlan {
+  int capacity;   // keys a table row can name
+  int chunks;     // blocks of query heads per key-value head
+  int q_pairs;    // q may be read two elements at a time
+  int o_quads;    // o may be written four elements at a time
+  float* partial; // [2 CTAs][rows][DP]
+  float2* ml;     // [2 CTAs][rows] maximum (log2 units) and sum
+  int* counters;  // [CTAs]
+};
+
+// Scores in log2 units: raw is q.k; with a cap, raw becomes tanh(raw * pre).
+struct PaScore {
+  float pre, mul;
+  bool cap;
+  __device__ PaScore(const th_paged_attention_args& p) {
+    cap = p.softcap > 0.f;
+    pre = cap ? p.scale / p.softcap : 1.f;
+    mul = (cap ? p.softcap : p.scale) * PA_LOG2E;
+  }
+  __device__ __forceinline__ float raw(float x) const { return cap ? tanhf(x * pre) : x; }
+};
+
+// --------------------------------------------------------------- 2-byte types
+// Transposed products, so that keys are the 16 rows of an mma and up to 8 NT
+// query heads its columns: S^T = K Q^T with K by ldmatrix, O^T += V^T P^T with
+// V by ldmatrix.trans; the 8x8 blocks of P^T are transposed in registers.  The
+// weights p are kept as a sum of two 16-bit numbers (p's rounding to 8 or 11
+// bits and the rounding of the rest): one rounding alone would add as much
+// error as the output's own; the second product costs no memory traffic.
+template <typename T_, int DP_, int NT, int KB_, int S_, int CTAS_>
+struct PaMma {
+  using T = T_;
+  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16;
+  static constexpr int SLOT = KB * DP * ES * 2, SHARED = 0;
+  static_assert(ROWS <= KB, "a warp's accumulator is joined through one block of its ring");
+  float o[DP / 16][NT][4], m[NT][2], l[NT][2];
+  uint32_t q[DP / 16][NT][2];
+
+  // 16-byte chunk c of row r: 8 consecutive rows of one chunk fall into distinct banks
+  static __device__ __forceinline__ int swz(int r, int c) { return c ^ (r & 7); }
+  static __device__ __forceinline__ int spill_at(int row, int d) { return row * DP + (d ^ (((row >> 1) & 3) << 3)); }
+
+  __device__ __forceinline__ void start(const th_paged_attention_args& p, const PaPlan& x, const T* qb, int rows, uint8_t*) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const T* src = qb + r * p.q_head;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = kk * 16 + e * 8 + 2 * t;
+          uint32_t v = 0;
+          if (r < rows && c < p.head_dim) {
+            if (x.q_pairs) v = *reinterpret_cast<const uint32_t*>(src + c);
+            else v = (uint32_t)*reinterpret_cast<const uint16_t*>(src + c) | ((uint32_t)*reinterpret_cast<const uint16_t*>(src + c + 1) << 16);
+          }
+          q[kk][nt][e] = v;
+        }
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dt][nt][e] = 0.f;
+  }
+
+  __device__ __forceinline__ void tile(uint32_t ks, uint32_t mask, int d, const PaScore& sc, uint8_t*) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const uint32_t vs = ks + KB * DP * ES;
+    float s[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+    float s2[4] = {0.f, 0.f, 0.f, 0.f};  // a second chain where there is only one
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      if (kk * 16 >= d) break;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t a[4];
+        const int r = mt * 16 + (lane & 15);
+        ldsm_x4(ks + r * (DP * ES) + swz(r, kk * 2 + (lane >> 4)) * 16, a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (MT * NT == 1 && (kk & 1)) mma16816<T>(s2, a, q[kk][nt][0], q[kk][nt][1]);
+          else mma16816<T>(s[mt][nt], a, q[kk][nt][0], q[kk][nt][1]);
+        }
+      }
+    }
+    if (MT * NT == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][0][e] += s2[e];
+    }
+    float mx[NT][2];
+    bool grew = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mx[nt][0] = m[nt][0];
+      mx[nt][1] = m[nt][1];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[mt][nt][e] = sc.raw(s[mt][nt][e]);
+          const bool live = (mask >> (mt * 16 + g + (e >> 1) * 8)) & 1;
+          mx[nt][e & 1] = fmaxf(mx[nt][e & 1], live ? s[mt][nt][e] * sc.mul : -INFINITY);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
+        grew |= mx[nt][e] > m[nt][e];
+      }
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          f[e] = m[nt][e] == -INFINITY ? 0.f : ex2_fast(m[nt][e] - mx[nt][e]);
+          l[nt][e] *= f[e];
+          m[nt][e] = mx[nt][e];
+        }
+#pragma unroll
+        for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[dt][nt][e] *= f[e & 1];
+      }
+    }
+    uint32_t hi[MT][NT][2], lo[MT][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const bool live = (mask >> (mt * 16 + g + r * 8)) & 1;
+          const float p0 = live ? ex2_fast(fmaf(s[mt][nt][2 * r], sc.mul, -m0)) : 0.f;
+          const float p1 = live ? ex2_fast(fmaf(s[mt][nt][2 * r + 1], sc.mul, -m1)) : 0.f;
+          l[nt][0] += p0;
+          l[nt][1] += p1;
+          hi[mt][nt][r] = movmatrix(pack2<T>(p0, p1));
+          lo[mt][nt][r] = movmatrix(pack2<T>(p0 - round_to<T>(p0), p1 - round_to<T>(p1)));
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+      if (dt * 16 >= d) break;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t a[4];
+        const int r = mt * 16 + (lane & 7) + ((lane >> 4) << 3);
+        ldsm_x4_trans(vs + r * (DP * ES) + swz(r, dt * 2 + ((lane >> 3) & 1)) * 16, a);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<T>(o[dt][nt], a, hi[mt][nt][0], hi[mt][nt][1]);
+          mma16816<T>(o[dt][nt], a, lo[mt][nt][0], lo[mt][nt][1]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void spill(float* dst, float2* ml) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (g == 0) ml[nt * 8 + 2 * t + e] = make_float2(m[nt][e], sum);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[spill_at(nt * 8 + 2 * t + (e & 1), dt * 16 + g + (e >> 1) * 8)] = o[dt][nt][e];
+    }
+  }
+};
+
+// --------------------------------------------------------------------- fp32
+// 8 keys per warp block: four lanes share a key's dot products (one 16-byte
+// chunk in four each), then every lane owns DP/32 elements of the output.
+template <int DP_, int NH, int S_, int CTAS_>
+struct PaSimt {
+  using T = float;
+  static constexpr int DP = DP_, KB = 8, S = S_, CTAS = CTAS_, ROWS = NH, ES = 4, EL = DP / 32;
+  static constexpr int SLOT = KB * DP * ES * 2, SHARED = (NH * DP + PA_WARPS * KB * NH) * 4;
+  static_assert(ROWS <= KB * 2, "a warp's accumulator is joined through one block of its ring");
+  float o[NH][EL], m[NH], l[NH];
+
+  // rows of odd parity swap the halves of each 128 bytes: 8 lanes on two rows hit distinct banks
+  static __device__ __forceinline__ int swz(int r, int c) { return c ^ ((r & 1) << 2); }
+  static __device__ __forceinline__ int spill_at(int row, int d) { return row * DP + d; }
+  // element of the head that slot e of this lane holds
+  static __device__ __forceinline__ int elem(int lane, int e) {
+    return DP == 256 ? (e >> 2) * 128 + lane * 4 + (e & 3) : lane * EL + e;
+  }
+
+  __device__ __forceinline__ void start(const th_paged_attention_args& p, const PaPlan&, const T* qb, int rows, uint8_t* shared) {
+    float* qs = reinterpret_cast<float*>(shared);
+    for (int i = threadIdx.x; i < NH * DP; i += PA_WARPS * 32) {
+      const int r = i / DP, c = i % DP;
+      qs[i] = r < rows && c < p.head_dim ? qb[r * p.q_head + c] : 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int e = 0; e < EL; ++e) o[h][e] = 0.f;
+    }
+    __syncthreads();  // every warp starts an item at the same time
+  }
+
+  __device__ __forceinline__ void tile(uint32_t ks, uint32_t mask, int d, const PaScore& sc, uint8_t* shared) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const uint32_t vs = ks + KB * DP * ES, qs = smem_u32(shared);
+    float* ps = reinterpret_cast<float*>(shared) + NH * DP + (threadIdx.x >> 5) * (KB * NH);
+    float s[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) s[h] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      if (i * 16 >= d) break;
+      const int ch = i * 4 + c;
+      const float4 k = lds128(ks + r * (DP * ES) + swz(r, ch) * 16);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float4 q = lds128(qs + (h * DP + ch * 4) * 4);
+        s[h] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[h]))));
+      }
+    }
+    const bool live = (mask >> r) & 1;
+    float f[NH];
+    bool grew = false;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
+      s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
+      s[h] = sc.raw(s[h]);
+      float mx = fmaxf(m[h], live ? s[h] * sc.mul : -INFINITY);
+#pragma unroll
+      for (int w = 4; w < 32; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      f[h] = m[h] == -INFINITY ? 0.f : ex2_fast(m[h] - mx);
+      grew |= mx > m[h];
+      m[h] = mx;
+      const float p = live ? ex2_fast(fmaf(s[h], sc.mul, mx == -INFINITY ? 0.f : -mx)) : 0.f;
+      l[h] = fmaf(l[h], f[h], p);
+      if (c == 0) ps[r * NH + h] = p;
+    }
+    if (grew) {  // the maxima are the same in every lane
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < EL; ++e) o[h][e] *= f[h];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      float v[EL];
+      const uint32_t row = vs + j * (DP * ES);
+      if constexpr (EL == 2) {
+        const float2 x = lds64(row + swz(j, lane >> 1) * 16 + (lane & 1) * 8);
+        v[0] = x.x; v[1] = x.y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EL; e += 4) {
+          const float4 x = lds128(row + swz(j, lane + e * 8) * 16);
+          v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float p = ps[j * NH + h];
+#pragma unroll
+        for (int e = 0; e < EL; ++e) o[h][e] = fmaf(p, v[e], o[h][e]);
+      }
+    }
+    __syncwarp();  // ps is written again by the next block
+  }
+
+  __device__ __forceinline__ void spill(float* dst, float2* ml) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      float sum = l[h];
+#pragma unroll
+      for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      if (lane == 0) ml[h] = make_float2(m[h], sum);
+#pragma unroll
+      for (int e = 0; e < EL; ++e) dst[spill_at(h, elem(lane, e))] = o[h][e];
+    }
+  }
+};
+
+// ---------------------------------------------------------- the walk over tiles
+// Tiles of a sequence: at least one, so that an empty one still writes zeros.
+__device__ __forceinline__ int pa_tiles(int n, int tile) { return n <= tile ? 1 : (n - 1) / tile + 1; }
+__device__ __forceinline__ int pa_clean(int len, const PaPlan& x) { return min(max(len, 0), x.capacity); }
+__device__ __forceinline__ int pa_kept(int len, int window) { return window > 0 ? min(len, window) : len; }
+
+struct PaWalk {
+  int b, hc, t, nt, len, ahead;  // sequence, head block, tile, tiles, keys, the next sequence's length
+};
+
+__device__ __forceinline__ void pa_enter(PaWalk& w, const th_paged_attention_args& p, const PaPlan& x, int len, int tile) {
+  w.len = pa_clean(len, x);
+  w.nt = pa_tiles(pa_kept(w.len, p.window), tile);
+  w.ahead = w.b + 1 < p.batch ? p.lens[w.b + 1] : 0;  // fetched a sequence early: its latency is not waited for
+}
+
+__device__ __forceinline__ void pa_next(PaWalk& w, const th_paged_attention_args& p, const PaPlan& x, int items, int tile) {
+  if (++w.t < w.nt) return;
+  w.t = 0;
+  if (++w.hc < items) return;
+  w.hc = 0;
+  ++w.b;
+  if (w.b < p.batch) pa_enter(w, p, x, w.ahead, tile);
+}
+
+// CTA whose run [W c / G, W (c+1) / G) holds tile u.
+__device__ __forceinline__ int pa_owner(long long u, long long W, long long G) {
+  long long c = u * G / W;
+  while (W * (c + 1) / G <= u) ++c;
+  return (int)c;
+}
+
+template <typename T>
+__device__ __forceinline__ void pa_store4(T* o, float4 v, float f, int quads) {
+  const float r[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+  if (quads) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = make_float4(r[0], r[1], r[2], r[3]);
+    else *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(r[e]);
+  }
+}
+
+template <class P>
+__global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
+    paged_attention_kernel(const __grid_constant__ th_paged_attention_args p, const __grid_constant__ PaPlan x) {
+  using T = typename P::T;
+  constexpr int S = P::S, KB = P::KB, DP = P::DP, TILE = PA_WARPS * KB, CH = DP * P::ES / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int4 sm_meta[PA_WARPS][S];
+  __shared__ uint32_t sm_mask[PA_WARPS][S];
+  __shared__ float2 sm_ml[PA_WARPS][P::ROWS];
+  __shared__ int sm_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.hq / p.hkv, items = p.hkv * x.chunks, d = p.head_dim, dch = d * P::ES / 16;
   pdl_wait();
   pdl_trigger();
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = p.head_dim;
-  const int h = blockIdx.x % p.hq, b = blockIdx.x / p.hq, hk = h / (p.hq / p.hkv);
-  const int64_t room = (int64_t)p.table_cols * p.page_size;
-  int len = max(p.lens[b], 0);
-  if (len > room) {
-    if (threadIdx.x == 0) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
-    len = (int)room;
-  }
-  const T* q = (const T*)p.q + b * p.q_row + h * p.q_head;
-  float qr[8], acc[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    qr[e] = lane + 32 * e < d ? to_f32(q[lane + 32 * e]) : 0.f;
-    acc[e] = 0.f;
-  }
-  const int first = p.window > 0 ? max(0, len - p.window) : 0;
-  for (int j = first + warp; j < len; j += 4) {
-    const int col = j / p.page_size, slot = j - col * p.page_size;
-    const int page = p.table[b * p.ld_table + col];
-    if (page < 0 || page >= p.num_pages) {
-      if (lane == 0) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
-      continue;
+
+  // this CTA's run of tiles [u0, u1)
+  long long total = 0;
+  for (int base = 0; base < p.batch; base += 32) {
+    unsigned n = 0;  // 32 sequences of 2^26 tiles fit
+    if (base + lane < p.batch) {
+      const int len = p.lens[base + lane];
+      if (len > x.capacity && blockIdx.x == 0 && warp == 0) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
+      n = pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE);
     }
-    const T* k = (const T*)p.k_pages + page * p.k_page + hk * p.k_head + slot * p.k_slot;
-    const T* v = (const T*)p.v_pages + page * p.v_page + hk * p.v_head + slot * p.v_slot;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < d) s = fmaf(qr[e], to_f32(k[lane + 32 * e]), s);
-    s = warp_sum(s) * p.scale;
-    if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
-    const float mn = fmaxf(m, s), top = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - top), w = expf(s - top);
-    l = l * keep + w;
-    m = mn;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < d) acc[e] = acc[e] * keep + w * to_f32(v[lane + 32 * e]);
+    total += __reduce_add_sync(0xffffffffu, n);
   }
-  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+  const long long W = total * items, G = min((long long)gridDim.x, W);
+  const long long c = blockIdx.x;
+  if (c >= G) return;
+  const long long u0 = W * c / G;
+  const int n = (int)(W * (c + 1) / G - u0);
+  PaWalk w;
+  {
+    long long before = 0;
+    for (int base = 0;; base += 32) {
+      const int len = base + lane < p.batch ? p.lens[base + lane] : 0;
+      const int nt = base + lane < p.batch ? pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE) : 0;
+      unsigned incl = nt;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sm_o[warp][lane + 32 * e] = acc[e];
-  __syncthreads();
-  float mm = -INFINITY, ll = 0.f, f[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w]);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm_m[w] == -INFINITY ? 0.f : expf(sm_m[w] - mm);
-    ll += sm_l[w] * f[w];
+      for (int s = 1; s < 32; s *= 2) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, incl, s);
+        if (lane >= s) incl += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, (before + incl) * items > u0);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        w.b = base + src;
+        before += __shfl_sync(0xffffffffu, incl - nt, src);
+        pa_enter(w, p, x, __shfl_sync(0xffffffffu, len, src), TILE);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    const long long in = u0 - before * items;
+    w.hc = (int)(in / w.nt);
+    w.t = (int)(in - (long long)w.hc * w.nt);
   }
-  T* o = (T*)p.o + b * p.o_row + h * p.o_head;
-  for (int i = threadIdx.x; i < d; i += 128) {
-    float x = 0.f;
+
+  uint8_t* const ring = smem + warp * (S * P::SLOT);
+  uint8_t* const shared = smem + PA_WARPS * S * P::SLOT;
+  const uint32_t ring_u = smem_u32(ring);
+  const T* const kp = reinterpret_cast<const T*>(p.k_pages);
+  const T* const vp = reinterpret_cast<const T*>(p.v_pages);
+
+  // page and slot of key `lane` of this warp's block of the walk's tile (slot -1: no key)
+  auto fetch = [&](const PaWalk& k, int& page, int& slot) {
+    const int j = k.len - pa_kept(k.len, p.window) + k.t * TILE + warp * KB + lane;
+    slot = -1;
+    page = -1;
+    if (lane < KB && j < k.len) {
+      const int col = (int)((unsigned)j / (unsigned)p.page_size);
+      page = p.table[(int64_t)k.b * p.ld_table + col];
+      slot = j - col * p.page_size;
+    }
+  };
+  auto issue = [&](const PaWalk& k, int at, int page, int slot) {
+    const bool live = slot >= 0 && (unsigned)page < (unsigned)p.num_pages;
+    if (slot >= 0 && !live) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
+    const uint32_t mask = __ballot_sync(0xffffffffu, live);
+    if (!live) page = -1;
+    if (lane == 0) {
+      sm_meta[warp][at] = make_int4(k.b, k.hc, k.t, k.nt);
+      sm_mask[warp][at] = mask;
+    }
+    if (mask == 0) return;  // nothing of it is read
+    const int hk = k.hc / x.chunks;
+    const T* kb = kp + hk * p.k_head;
+    const T* vb = vp + hk * p.v_head;
+    const uint32_t dst = ring_u + at * P::SLOT;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) x += sm_o[w][i] * f[w];
-    o[i] = from_f32<T>(ll == 0.f ? 0.f : x / ll);
+    for (int i = 0; i < KB * CH / 32; ++i) {
+      const int id = i * 32 + lane, row = id / CH, ch = id % CH;
+      const int rp = __shfl_sync(0xffffffffu, page, row), rs = __shfl_sync(0xffffffffu, slot, row);
+      const bool ok = rp >= 0 && ch < dch;
+      const uint32_t to = dst + row * (DP * P::ES) + P::swz(row, ch) * 16;
+      const T* ka = kb + rp * p.k_page + rs * p.k_slot + ch * (16 / P::ES);
+      const T* va = vb + rp * p.v_page + rs * p.v_slot + ch * (16 / P::ES);
+      cp_async16(to, ok ? ka : kp, ok ? 16 : 0);
+      cp_async16(to + KB * DP * P::ES, ok ? va : vp, ok ? 16 : 0);
+    }
+  };
+
+  {  // fill the ring: all page ids first, then all copies
+    PaWalk ws[S - 1];
+    int page[S - 1], slot[S - 1];
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+      ws[s] = w;
+      if (s < n) {
+        fetch(w, page[s], slot[s]);
+        pa_next(w, p, x, items, TILE);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+      if (s < n) issue(ws[s], s, page[s], slot[s]);
+      cp_async_commit();
+    }
   }
-  if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.hq + h] = ll == 0.f ? -INFINITY : mm + logf(ll);
+  int page_n = -1, slot_n = -1;
+  if (S - 1 < n) fetch(w, page_n, slot_n);
+
+  P acc;
+  const PaScore sc(p);
+  int begin = 0;  // first tile of the current item that this CTA has
+  int at = 0, put = S - 1;
+  for (int i = 0; i < n; ++i) {
+    cp_async_wait<S - 2>();
+    __syncwarp();
+    if (i + S - 1 < n) issue(w, put, page_n, slot_n);
+    cp_async_commit();
+    if (i + S < n) {
+      pa_next(w, p, x, items, TILE);
+      fetch(w, page_n, slot_n);
+    }
+    const int4 meta = sm_meta[warp][at];
+    const int b = meta.x, hk = meta.y / x.chunks, r0 = (meta.y - hk * x.chunks) * P::ROWS;
+    const int rows = min(P::ROWS, group - r0), h0 = hk * group + r0;
+    if (i == 0 || meta.z == 0) {
+      begin = meta.z;
+      acc.start(p, x, reinterpret_cast<const T*>(p.q) + b * p.q_row + h0 * p.q_head, rows, shared);
+    }
+    const uint32_t mask = sm_mask[warp][at];
+    if (mask) acc.tile(ring_u + at * P::SLOT, mask, d, sc, shared);
+
+    if (meta.z == meta.w - 1 || i == n - 1) {
+      // join the warps through the blocks they have just read
+      __syncwarp();
+      acc.spill(reinterpret_cast<float*>(ring + at * P::SLOT), sm_ml[warp]);
+      __syncthreads();
+      const bool whole = begin == 0 && meta.z == meta.w - 1;
+      const int mine = 2 * (int)c + (begin == 0 ? 1 : 0);
+      const int quads = d / 4;
+      for (int e = tid; e < rows * quads; e += PA_WARPS * 32) {
+        const int r = e / quads, dd = (e - r * quads) * 4;
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int k = 0; k < PA_WARPS; ++k) mm = fmaxf(mm, sm_ml[k][r].x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < PA_WARPS; ++k) {
+          const float2 ml = sm_ml[k][r];
+          const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - mm);
+          const float4 y = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(smem + (k * S + at) * P::SLOT) + P::spill_at(r, dd));
+          // a warp without keys holds no maximum; its accumulator is zero
+          v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+          ll = fmaf(f, ml.y, ll);
+        }
+        if (whole) {
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          T* o = reinterpret_cast<T*>(p.o) + b * p.o_row + (h0 + r) * p.o_head + dd;
+          pa_store4(o, v, inv, x.o_quads);
+          if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+        } else {
+          *reinterpret_cast<float4*>(x.partial + ((int64_t)mine * P::ROWS + r) * DP + dd) = v;
+          if (dd == 0) x.ml[(int64_t)mine * P::ROWS + r] = make_float2(mm, ll);
+        }
+      }
+      if (!whole) {
+        // the CTAs on this item: those whose runs meet its tiles
+        const long long ub = u0 + i - meta.z, ue = ub + meta.w - 1;
+        const int c0 = pa_owner(ub, W, G), c1 = pa_owner(ue, W, G);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) sm_last = atomicAdd(x.counters + c0, 1) == c1 - c0;
+        __syncthreads();
+        if (sm_last) {
+          __threadfence();
+          if (tid == 0) x.counters[c0] = 0;  // ready for the next call
+          for (int e = tid; e < rows * quads; e += PA_WARPS * 32) {
+            const int r = e / quads, dd = (e - r * quads) * 4;
+            float mm = -INFINITY, ll = 0.f;
+#pragma unroll 8
+            for (int k = c0; k <= c1; ++k)
+              mm = fmaxf(mm, __ldcg(&x.ml[(2 * (int64_t)k + (k == c0)) * P::ROWS + r].x));
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int k = c0; k <= c1; ++k) {
+              const int64_t row = (2 * (int64_t)k + (k == c0)) * P::ROWS + r;
+              const float2 ml = __ldcg(x.ml + row);
+              const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - mm);
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(x.partial + row * DP + dd));
+              v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+              ll = fmaf(f, ml.y, ll);
+            }
+            const float inv = ll == 0.f ? 0.f : 1.f / ll;
+            T* o = reinterpret_cast<T*>(p.o) + b * p.o_row + (h0 + r) * p.o_head + dd;
+            pa_store4(o, v, inv, x.o_quads);
+            if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    at = at + 1 == S ? 0 : at + 1;
+    put = put + 1 == S ? 0 : put + 1;
+  }
+}
+
+// --------------------------------------------------------------------- host
+template <class P>
+struct PaKind { using type = P; };
+
+// Calls f with the kernel's kind for these heads.  The head is padded to 64,
+// 128 or 256 elements in shared memory (the padding is not read from memory);
+// a kind holds as many query heads of a group as its registers allow.
+template <typename F>
+static auto pa_dispatch(int dtype, int head_dim, int group, F&& f) {
+  auto two = [&](auto tag) {
+    using T = decltype(tag);
+    if (head_dim <= 64) {
+      if (group <= 8) return f(PaKind<PaMma<T, 64, 1, 32, 3, 2>>{});
+      if (group <= 16) return f(PaKind<PaMma<T, 64, 2, 32, 3, 2>>{});
+      return f(PaKind<PaMma<T, 64, 4, 32, 3, 2>>{});
+    }
+    if (head_dim <= 128) {
+      if (group <= 8) return f(PaKind<PaMma<T, 128, 1, 16, 3, 2>>{});
+      if (group <= 16) return f(PaKind<PaMma<T, 128, 2, 16, 3, 2>>{});
+      return f(PaKind<PaMma<T, 128, 4, 32, 3, 1>>{});
+    }
+    if (group <= 8) return f(PaKind<PaMma<T, 256, 1, 16, 3, 1>>{});
+    return f(PaKind<PaMma<T, 256, 2, 16, 3, 1>>{});
+  };
+  if (dtype == TH_BF16) return two(__nv_bfloat16{});
+  if (dtype == TH_F16) return two(__half{});
+  if (head_dim <= 64) {
+    if (group == 1) return f(PaKind<PaSimt<64, 1, 4, 2>>{});
+    if (group <= 4) return f(PaKind<PaSimt<64, 4, 4, 2>>{});
+    return f(PaKind<PaSimt<64, 8, 4, 2>>{});
+  }
+  if (head_dim <= 128) {
+    if (group == 1) return f(PaKind<PaSimt<128, 1, 3, 2>>{});
+    if (group <= 4) return f(PaKind<PaSimt<128, 4, 3, 2>>{});
+    return f(PaKind<PaSimt<128, 8, 3, 2>>{});
+  }
+  if (group == 1) return f(PaKind<PaSimt<256, 1, 3, 1>>{});
+  return f(PaKind<PaSimt<256, 4, 3, 1>>{});
+}
+
+static size_t pa_round(size_t n) { return (n + 255) / 256 * 256; }
+
+template <class P>
+static size_t pa_workspace(PaPlan* x, void* base) {
+  const size_t ctas = (size_t)sm_count() * P::CTAS;
+  const size_t counters = pa_round(ctas * 4), ml = pa_round(2 * ctas * P::ROWS * 8), partial = 2 * ctas * P::ROWS * P::DP * 4;
+  if (x) {
+    uint8_t* b = static_cast<uint8_t*>(base);
+    x->counters = reinterpret_cast<int*>(b);
+    x->ml = reinterpret_cast<float2*>(b + counters);
+    x->partial = reinterpret_cast<float*>(b + counters + ml);
+  }
+  return counters + ml + partial;
+}
+
+static bool pa_supported(int hq, int hkv, int head_dim, int dtype) {
+  return hq > 0 && hkv > 0 && hq % hkv == 0 && dtype >= TH_F32 && dtype <= TH_F16 && head_dim > 0 && head_dim <= 256 &&
+         head_dim * elem_bytes(dtype) % 16 == 0;
+}
+
+template <class P>
+static int pa_launch(const th_paged_attention_args* a, PaPlan x, cudaStream_t st) {
+  if (a->workspace_bytes < pa_workspace<P>(&x, a->workspace))
+    return fail(TH_EINVAL, "th_paged_attention: workspace %zu B < %zu B", a->workspace_bytes, pa_workspace<P>(nullptr, nullptr));
+  x.chunks = (a->hq / a->hkv + P::ROWS - 1) / P::ROWS;
+  const size_t smem = (size_t)PA_WARPS * P::S * P::SLOT + P::SHARED;
+  if (int rc = smem_limit(paged_attention_kernel<P>, smem, "th_paged_attention")) return rc;
+  launch_pdl(paged_attention_kernel<P>, dim3(sm_count() * P::CTAS), dim3(PA_WARPS * 32), smem, st, *a, x);
+  return check_launch("th_paged_attention");
 }
 
 }  // namespace th
 
 extern "C" size_t th_paged_attention_workspace_size(int32_t hq, int32_t hkv, int32_t head_dim, int32_t dtype) {
   using namespace th;
-  if (hq <= 0 || hkv <= 0 || hq % hkv || head_dim <= 0 || head_dim > 256 || dtype < TH_F32 || dtype > TH_F16 ||
-      head_dim * elem_bytes(dtype) % 16)
-    return 0;
-  return 16;
+  if (!pa_supported(hq, hkv, head_dim, dtype)) return 0;
+  return pa_dispatch(dtype, head_dim, hq / hkv, [](auto k) { return pa_workspace<typename decltype(k)::type>(nullptr, nullptr); });
 }
 
 extern "C" int th_paged_attention(const th_paged_attention_args* a, void* stream) {
@@ -92,22 +729,21 @@ extern "C" int th_paged_attention(const th_paged_attention_args* a, void* stream
   if (a->page_size <= 0 || a->num_pages <= 0 || a->table_cols <= 0 || a->ld_table < (a->batch > 1 ? a->table_cols : 0))
     return fail(TH_EINVAL, "th_paged_attention: bad cache shape");
   if (a->dtype < TH_F32 || a->dtype > TH_F16) return fail(TH_EDTYPE, "th_paged_attention: bad dtype %d", a->dtype);
-  const int eb = elem_bytes(a->dtype);
-  if (a->head_dim <= 0 || a->head_dim > 256 || a->head_dim * eb % 16)
+  if (!pa_supported(a->hq, a->hkv, a->head_dim, a->dtype))
     return fail(TH_EUNSUPPORTED, "th_paged_attention: head_dim %d (at most 256, rows of a multiple of 16 bytes)", a->head_dim);
   if (a->window < 0 || !(a->softcap >= 0.f)) return fail(TH_EINVAL, "th_paged_attention: negative window or softcap");
+  const int eb = elem_bytes(a->dtype);
   const int64_t strides[] = {a->k_page, a->k_head, a->k_slot, a->v_page, a->v_head, a->v_slot};
   for (int64_t s : strides)
     if (s * eb % 16) return fail(TH_EALIGN, "th_paged_attention: pool strides must be multiples of 16 bytes");
   if (!aligned16(a->k_pages) || !aligned16(a->v_pages) || !aligned16(a->workspace))
     return fail(TH_EALIGN, "th_paged_attention: pools and workspace must be 16-byte aligned");
-  const size_t need = th_paged_attention_workspace_size(a->hq, a->hkv, a->head_dim, a->dtype);
-  if (a->workspace_bytes < need)
-    return fail(TH_EINVAL, "th_paged_attention: workspace %zu B < %zu B", a->workspace_bytes, need);
+  PaPlan x{};
+  const int64_t cap = (int64_t)a->table_cols * a->page_size;
+  x.capacity = (int)(cap < INT32_MAX - 4096 ? cap : INT32_MAX - 4096);
+  x.q_pairs = reinterpret_cast<uintptr_t>(a->q) % 4 == 0 && a->q_row % 2 == 0 && a->q_head % 2 == 0;
+  x.o_quads = reinterpret_cast<uintptr_t>(a->o) % (4 * eb) == 0 && a->o_row % 4 == 0 && a->o_head % 4 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(a->batch * a->hq));
-  if (a->dtype == TH_F32) launch_pdl(paged_attention_kernel<float>, grid, dim3(128), 0, st, *a);
-  else if (a->dtype == TH_BF16) launch_pdl(paged_attention_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, *a);
-  else launch_pdl(paged_attention_kernel<__half>, grid, dim3(128), 0, st, *a);
-  return check_launch("th_paged_attention");
+  return pa_dispatch(a->dtype, a->head_dim, a->hq / a->hkv,
+                     [&](auto k) { return pa_launch<typename decltype(k)::type>(a, x, st); });
 }
