@@ -58,6 +58,11 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ int atom_add_acq_rel(int* p, int v) {
+  int old;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
 __device__ __forceinline__ float4 lds128(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -73,6 +78,8 @@ __device__ __forceinline__ float2 lds64(uint32_t addr) {
 struct PaPlan {
   int capacity;   // keys a table row can name
   int chunks;     // blocks of query heads per key-value head
+  int page_shift; // log2 of the page size, or -1
+  int same;       // both pools have the same strides
   int q_pairs;    // q may be read two elements at a time
   int o_quads;    // o may be written four elements at a time
   float* partial; // [2 CTAs][rows][DP]
@@ -80,7 +87,17 @@ struct PaPlan {
   int* counters;  // [CTAs]
 };
 
-// Scores in log2 units: raw is q.k; with a cap, raw becomes tanh(raw * pre).
+// tanh from one exponential and one reciprocal; below 1/4, where 1 - 2/(1+e^2x)
+// would lose the small result's bits, the first four terms of its series.
+// Within 5e-7 of the result; used where the output has at most 11 bits.
+__device__ __forceinline__ float tanh_ex2(float x) {
+  const float big = 1.f - __fdividef(2.f, 1.f + ex2_fast(fminf(x * (2.f * PA_LOG2E), 126.f)));
+  const float y = x * x;
+  const float small = x * fmaf(y, fmaf(y, fmaf(y, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  return fabsf(x) < 0.25f ? small : big;
+}
+
+// Scores in log2 units are raw * mul: raw is q.k, or with a cap tanh(q.k * pre).
 struct PaScore {
   float pre, mul;
   bool cap;
@@ -89,7 +106,11 @@ struct PaScore {
     pre = cap ? p.scale / p.softcap : 1.f;
     mul = (cap ? p.softcap : p.scale) * PA_LOG2E;
   }
-  __device__ __forceinline__ float raw(float x) const { return cap ? tanhf(x * pre) : x; }
+  template <int ES>
+  __device__ __forceinline__ float raw(float x) const {
+    if (!cap) return x;
+    return ES == 4 ? tanhf(x * pre) : tanh_ex2(x * pre);
+  }
 };
 
 // --------------------------------------------------------------- 2-byte types
@@ -102,9 +123,10 @@ struct PaScore {
 template <typename T_, int DP_, int NT, int KB_, int S_, int CTAS_>
 struct PaMma {
   using T = T_;
-  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16;
+  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16, FLY = NT == 1 ? 16 : 8;
   static constexpr int SLOT = KB * DP * ES * 2, SHARED = 0;
-  static_assert(ROWS <= KB, "a warp's accumulator is joined through one block of its ring");
+  static constexpr int PASS = ROWS < KB ? ROWS : KB;  // rows of the accumulator that one block of the ring holds
+  static_assert(PASS % 8 == 0, "whole mma columns");
   float o[DP / 16][NT][4], m[NT][2], l[NT][2];
   uint32_t q[DP / 16][NT][2];
 
@@ -112,24 +134,32 @@ struct PaMma {
   static __device__ __forceinline__ int swz(int r, int c) { return c ^ (r & 7); }
   static __device__ __forceinline__ int spill_at(int row, int d) { return row * DP + (d ^ (((row >> 1) & 3) << 3)); }
 
-  __device__ __forceinline__ void start(const th_paged_attention_args& p, const PaPlan& x, const T* qb, int rows, uint8_t*) {
+  __device__ __forceinline__ void load_q(const th_paged_attention_args& p, const PaPlan& x, const T* qb, int rows, uint8_t*) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    auto fill = [&](auto read) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        const T* src = qb + r * p.q_head;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = kk * 16 + e * 8 + 2 * t;
+            q[kk][nt][e] = r < rows && c < p.head_dim ? read(src + c) : 0u;
+          }
+      }
+    };
+    if (x.q_pairs) fill([](const T* a) { return *reinterpret_cast<const uint32_t*>(a); });
+    else fill([](const T* a) {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(a);
+      return (uint32_t)h[0] | ((uint32_t)h[1] << 16);
+    });
+  }
+
+  __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      const T* src = qb + r * p.q_head;
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = kk * 16 + e * 8 + 2 * t;
-          uint32_t v = 0;
-          if (r < rows && c < p.head_dim) {
-            if (x.q_pairs) v = *reinterpret_cast<const uint32_t*>(src + c);
-            else v = (uint32_t)*reinterpret_cast<const uint16_t*>(src + c) | ((uint32_t)*reinterpret_cast<const uint16_t*>(src + c + 1) << 16);
-          }
-          q[kk][nt][e] = v;
-        }
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
@@ -181,7 +211,7 @@ struct PaMma {
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[mt][nt][e] = sc.raw(s[mt][nt][e]);
+          s[mt][nt][e] = sc.template raw<ES>(s[mt][nt][e]);
           const bool live = (mask >> (mt * 16 + g + (e >> 1) * 8)) & 1;
           mx[nt][e & 1] = fmaxf(mx[nt][e & 1], live ? s[mt][nt][e] * sc.mul : -INFINITY);
         }
@@ -242,10 +272,10 @@ struct PaMma {
     }
   }
 
-  __device__ __forceinline__ void spill(float* dst, float2* ml) {
+  __device__ __forceinline__ void stats(float2* ml) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sum = l[nt][e];
@@ -253,10 +283,17 @@ struct PaMma {
         for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
         if (g == 0) ml[nt * 8 + 2 * t + e] = make_float2(m[nt][e], sum);
       }
+  }
+  __device__ __forceinline__ void spill(float* dst, int pass) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt / (PASS / 8) != pass) continue;
 #pragma unroll
       for (int dt = 0; dt < DP / 16; ++dt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dst[spill_at(nt * 8 + 2 * t + (e & 1), dt * 16 + g + (e >> 1) * 8)] = o[dt][nt][e];
+        for (int e = 0; e < 4; ++e)
+          dst[spill_at((nt * 8) % PASS + 2 * t + (e & 1), dt * 16 + g + (e >> 1) * 8)] = o[dt][nt][e];
     }
   }
 };
@@ -267,8 +304,9 @@ struct PaMma {
 template <int DP_, int NH, int S_, int CTAS_>
 struct PaSimt {
   using T = float;
-  static constexpr int DP = DP_, KB = 8, S = S_, CTAS = CTAS_, ROWS = NH, ES = 4, EL = DP / 32;
+  static constexpr int DP = DP_, KB = 8, S = S_, CTAS = CTAS_, ROWS = NH, ES = 4, EL = DP / 32, FLY = 16;
   static constexpr int SLOT = KB * DP * ES * 2, SHARED = (NH * DP + PA_WARPS * KB * NH) * 4;
+  static constexpr int PASS = ROWS;
   static_assert(ROWS <= KB * 2, "a warp's accumulator is joined through one block of its ring");
   float o[NH][EL], m[NH], l[NH];
 
@@ -280,12 +318,16 @@ struct PaSimt {
     return DP == 256 ? (e >> 2) * 128 + lane * 4 + (e & 3) : lane * EL + e;
   }
 
-  __device__ __forceinline__ void start(const th_paged_attention_args& p, const PaPlan&, const T* qb, int rows, uint8_t* shared) {
+  // between two block-wide barriers
+  __device__ __forceinline__ void load_q(const th_paged_attention_args& p, const PaPlan&, const T* qb, int rows, uint8_t* shared) {
     float* qs = reinterpret_cast<float*>(shared);
     for (int i = threadIdx.x; i < NH * DP; i += PA_WARPS * 32) {
       const int r = i / DP, c = i % DP;
       qs[i] = r < rows && c < p.head_dim ? qb[r * p.q_head + c] : 0.f;
     }
+  }
+
+  __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       m[h] = -INFINITY;
@@ -293,7 +335,6 @@ struct PaSimt {
 #pragma unroll
       for (int e = 0; e < EL; ++e) o[h][e] = 0.f;
     }
-    __syncthreads();  // every warp starts an item at the same time
   }
 
   __device__ __forceinline__ void tile(uint32_t ks, uint32_t mask, int d, const PaScore& sc, uint8_t* shared) {
@@ -321,7 +362,7 @@ struct PaSimt {
     for (int h = 0; h < NH; ++h) {
       s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
       s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
-      s[h] = sc.raw(s[h]);
+      s[h] = sc.template raw<ES>(s[h]);
       float mx = fmaxf(m[h], live ? s[h] * sc.mul : -INFINITY);
 #pragma unroll
       for (int w = 4; w < 32; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -363,17 +404,21 @@ struct PaSimt {
     __syncwarp();  // ps is written again by the next block
   }
 
-  __device__ __forceinline__ void spill(float* dst, float2* ml) {
-    const int lane = threadIdx.x & 31;
+  __device__ __forceinline__ void stats(float2* ml) {
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       float sum = l[h];
 #pragma unroll
       for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      if (lane == 0) ml[h] = make_float2(m[h], sum);
+      if ((threadIdx.x & 31) == 0) ml[h] = make_float2(m[h], sum);
+    }
+  }
+  __device__ __forceinline__ void spill(float* dst, int) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
       for (int e = 0; e < EL; ++e) dst[spill_at(h, elem(lane, e))] = o[h][e];
-    }
   }
 };
 
@@ -402,12 +447,22 @@ __device__ __forceinline__ void pa_next(PaWalk& w, const th_paged_attention_args
   if (w.b < p.batch) pa_enter(w, p, x, w.ahead, tile);
 }
 
-// CTA whose run [W c / G, W (c+1) / G) holds tile u.
-__device__ __forceinline__ int pa_owner(long long u, long long W, long long G) {
-  long long c = u * G / W;
-  while (W * (c + 1) / G <= u) ++c;
-  return (int)c;
-}
+// W tiles over G CTAs: the first `extra` CTAs take `each` + 1, the others `each`.
+struct PaSplit {
+  long long each, extra;
+  static __device__ __forceinline__ long long div(long long a, long long b) {  // a, b >= 0
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+  }
+  __device__ PaSplit(long long W, int G) {
+    each = div(W, G);
+    extra = W - each * G;
+  }
+  __device__ __forceinline__ long long first(int c) const { return c * each + min((long long)c, extra); }
+  __device__ __forceinline__ int owner(long long u) const {
+    const long long bend = extra * (each + 1);
+    return (int)(u < bend ? div(u, each + 1) : extra + div(u - bend, each));
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ void pa_store4(T* o, float4 v, float f, int quads) {
@@ -436,7 +491,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
   pdl_wait();
   pdl_trigger();
 
-  // this CTA's run of tiles [u0, u1)
+  // this CTA's run of tiles [u0, u0 + n)
   long long total = 0;
   for (int base = 0; base < p.batch; base += 32) {
     unsigned n = 0;  // 32 sequences of 2^26 tiles fit
@@ -447,17 +502,20 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
     }
     total += __reduce_add_sync(0xffffffffu, n);
   }
-  const long long W = total * items, G = min((long long)gridDim.x, W);
-  const long long c = blockIdx.x;
+  const long long W = total * items;
+  // as few CTAs as still finish in the same number of tiles: fewer parts to join
+  const long long most = PaSplit::div(W + gridDim.x - 1, gridDim.x);
+  const int G = (int)PaSplit::div(W + most - 1, most), c = blockIdx.x;
   if (c >= G) return;
-  const long long u0 = W * c / G;
-  const int n = (int)(W * (c + 1) / G - u0);
+  const PaSplit split(W, G);
+  const long long u0 = split.first(c);
+  const int n = (int)(split.first(c + 1) - u0);
   PaWalk w;
   {
     long long before = 0;
     for (int base = 0;; base += 32) {
       const int len = base + lane < p.batch ? p.lens[base + lane] : 0;
-      const int nt = base + lane < p.batch ? pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE) : 0;
+      const unsigned nt = base + lane < p.batch ? pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE) : 0;
       unsigned incl = nt;
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) {
@@ -475,7 +533,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
     const long long in = u0 - before * items;
-    w.hc = (int)(in / w.nt);
+    w.hc = (int)PaSplit::div(in, w.nt);
     w.t = (int)(in - (long long)w.hc * w.nt);
   }
 
@@ -491,41 +549,57 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
     slot = -1;
     page = -1;
     if (lane < KB && j < k.len) {
-      const int col = (int)((unsigned)j / (unsigned)p.page_size);
+      const int col = x.page_shift >= 0 ? j >> x.page_shift : (int)((unsigned)j / (unsigned)p.page_size);
       page = p.table[(int64_t)k.b * p.ld_table + col];
       slot = j - col * p.page_size;
     }
   };
+  // Eight lanes copy 128 bytes of one row, so a warp copies four rows at a
+  // time and a lane needs the addresses of only KB/4 rows.
+  const int sub = lane & 7;
   auto issue = [&](const PaWalk& k, int at, int page, int slot) {
     const bool live = slot >= 0 && (unsigned)page < (unsigned)p.num_pages;
     if (slot >= 0 && !live) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
     const uint32_t mask = __ballot_sync(0xffffffffu, live);
-    if (!live) page = -1;
     if (lane == 0) {
       sm_meta[warp][at] = make_int4(k.b, k.hc, k.t, k.nt);
       sm_mask[warp][at] = mask;
     }
     if (mask == 0) return;  // nothing of it is read
-    const int hk = k.hc / x.chunks;
-    const T* kb = kp + hk * p.k_head;
-    const T* vb = vp + hk * p.v_head;
-    const uint32_t dst = ring_u + at * P::SLOT;
+    const int hk = x.chunks == 1 ? k.hc : k.hc / x.chunks;
+    const long long ko = live ? page * p.k_page + slot * p.k_slot + hk * p.k_head : 0;
+    const long long vo = live && !x.same ? page * p.v_page + slot * p.v_slot + hk * p.v_head : 0;
+    const uint32_t dst = ring_u + at * P::SLOT + (lane >> 3) * (DP * P::ES);
 #pragma unroll
-    for (int i = 0; i < KB * CH / 32; ++i) {
-      const int id = i * 32 + lane, row = id / CH, ch = id % CH;
-      const int rp = __shfl_sync(0xffffffffu, page, row), rs = __shfl_sync(0xffffffffu, slot, row);
-      const bool ok = rp >= 0 && ch < dch;
-      const uint32_t to = dst + row * (DP * P::ES) + P::swz(row, ch) * 16;
-      const T* ka = kb + rp * p.k_page + rs * p.k_slot + ch * (16 / P::ES);
-      const T* va = vb + rp * p.v_page + rs * p.v_slot + ch * (16 / P::ES);
-      cp_async16(to, ok ? ka : kp, ok ? 16 : 0);
-      cp_async16(to + KB * DP * P::ES, ok ? va : vp, ok ? 16 : 0);
+    for (int i = 0; i < KB / 4; ++i) {
+      const int row = i * 4 + (lane >> 3);
+      const long long ki = __shfl_sync(0xffffffffu, ko, row);
+      const long long vi = x.same ? ki : __shfl_sync(0xffffffffu, vo, row);
+      const bool ok = (mask >> row) & 1;
+      const T* ka = kp + ki + sub * (16 / P::ES);
+      const T* va = vp + vi + sub * (16 / P::ES);
+#pragma unroll
+      for (int h = 0; h < CH / 8; ++h) {
+        const int bytes = ok && h * 8 + sub < dch ? 16 : 0;  // 0: the copy fills zeros and reads nothing
+        const uint32_t to = dst + i * 4 * (DP * P::ES) + h * 128 + P::swz(row, sub) * 16;
+        cp_async16(to, bytes ? ka + h * (128 / P::ES) : kp, bytes);
+        cp_async16(to + KB * DP * P::ES, bytes ? va + h * (128 / P::ES) : vp, bytes);
+      }
     }
+  };
+
+  P acc;
+  const PaScore sc(p);
+  // the query heads of item (b, hc)
+  auto load_q = [&](int b, int hc) {
+    const int hk = x.chunks == 1 ? hc : hc / x.chunks, r0 = (hc - hk * x.chunks) * P::ROWS;
+    acc.load_q(p, x, reinterpret_cast<const T*>(p.q) + b * p.q_row + (hk * group + r0) * p.q_head, min(P::ROWS, group - r0), shared);
   };
 
   {  // fill the ring: all page ids first, then all copies
     PaWalk ws[S - 1];
     int page[S - 1], slot[S - 1];
+    const int b0 = w.b, hc0 = w.hc;
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
       ws[s] = w;
@@ -534,18 +608,19 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
         pa_next(w, p, x, items, TILE);
       }
     }
+    load_q(b0, hc0);
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
       if (s < n) issue(ws[s], s, page[s], slot[s]);
       cp_async_commit();
     }
+    acc.reset();
+    if (P::SHARED) __syncthreads();
   }
   int page_n = -1, slot_n = -1;
   if (S - 1 < n) fetch(w, page_n, slot_n);
 
-  P acc;
-  const PaScore sc(p);
-  int begin = 0;  // first tile of the current item that this CTA has
+  int begin = w.t;  // first tile of the current item that this CTA has
   int at = 0, put = S - 1;
   for (int i = 0; i < n; ++i) {
     cp_async_wait<S - 2>();
@@ -557,84 +632,109 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
       fetch(w, page_n, slot_n);
     }
     const int4 meta = sm_meta[warp][at];
-    const int b = meta.x, hk = meta.y / x.chunks, r0 = (meta.y - hk * x.chunks) * P::ROWS;
-    const int rows = min(P::ROWS, group - r0), h0 = hk * group + r0;
-    if (i == 0 || meta.z == 0) {
-      begin = meta.z;
-      acc.start(p, x, reinterpret_cast<const T*>(p.q) + b * p.q_row + h0 * p.q_head, rows, shared);
-    }
+    if (i == 0) begin = meta.z;
     const uint32_t mask = sm_mask[warp][at];
     if (mask) acc.tile(ring_u + at * P::SLOT, mask, d, sc, shared);
 
     if (meta.z == meta.w - 1 || i == n - 1) {
       // join the warps through the blocks they have just read
-      __syncwarp();
-      acc.spill(reinterpret_cast<float*>(ring + at * P::SLOT), sm_ml[warp]);
-      __syncthreads();
+      const int b = meta.x, hk = x.chunks == 1 ? meta.y : meta.y / x.chunks, r0 = (meta.y - hk * x.chunks) * P::ROWS;
+      const int rows = min(P::ROWS, group - r0), h0 = hk * group + r0, quads = d / 4;
       const bool whole = begin == 0 && meta.z == meta.w - 1;
-      const int mine = 2 * (int)c + (begin == 0 ? 1 : 0);
-      const int quads = d / 4;
-      for (int e = tid; e < rows * quads; e += PA_WARPS * 32) {
-        const int r = e / quads, dd = (e - r * quads) * 4;
-        float mm = -INFINITY, ll = 0.f;
+      const int mine = 2 * c + (begin == 0 ? 1 : 0);
+      auto finish = [&](int r, int dd, float4 v, float mm, float ll) {
+        T* o = reinterpret_cast<T*>(p.o) + b * p.o_row + (h0 + r) * p.o_head + dd;
+        pa_store4(o, v, ll == 0.f ? 0.f : 1.f / ll, x.o_quads);
+        if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+      };
+      acc.stats(sm_ml[warp]);
+      __syncwarp();
 #pragma unroll
-        for (int k = 0; k < PA_WARPS; ++k) mm = fmaxf(mm, sm_ml[k][r].x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int pass = 0; pass < (P::ROWS + P::PASS - 1) / P::PASS; ++pass) {
+        if (pass * P::PASS >= rows) break;
+        if (pass) __syncthreads();
+        acc.spill(reinterpret_cast<float*>(ring + at * P::SLOT), pass);
+        __syncthreads();
+        for (int e = tid; e < min(rows - pass * P::PASS, P::PASS) * quads; e += PA_WARPS * 32) {
+          const int rp = e / quads, dd = (e - rp * quads) * 4, r = pass * P::PASS + rp;
+          float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-        for (int k = 0; k < PA_WARPS; ++k) {
-          const float2 ml = sm_ml[k][r];
-          const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - mm);
-          const float4 y = *reinterpret_cast<const float4*>(
-              reinterpret_cast<const float*>(smem + (k * S + at) * P::SLOT) + P::spill_at(r, dd));
-          // a warp without keys holds no maximum; its accumulator is zero
-          v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
-          ll = fmaf(f, ml.y, ll);
+          for (int k = 0; k < PA_WARPS; ++k) mm = fmaxf(mm, sm_ml[k][r].x);
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < PA_WARPS; ++k) {
+            const float2 ml = sm_ml[k][r];
+            const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - mm);
+            const float4 y = *reinterpret_cast<const float4*>(
+                reinterpret_cast<const float*>(smem + (k * S + at) * P::SLOT) + P::spill_at(rp, dd));
+            v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+            ll = fmaf(f, ml.y, ll);
+          }
+          if (whole) {
+            finish(r, dd, v, mm, ll);
+          } else {
+            *reinterpret_cast<float4*>(x.partial + ((int64_t)mine * P::ROWS + r) * DP + dd) = v;
+            if (dd == 0) x.ml[(int64_t)mine * P::ROWS + r] = make_float2(mm, ll);
+          }
         }
-        if (whole) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          T* o = reinterpret_cast<T*>(p.o) + b * p.o_row + (h0 + r) * p.o_head + dd;
-          pa_store4(o, v, inv, x.o_quads);
-          if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
-        } else {
-          *reinterpret_cast<float4*>(x.partial + ((int64_t)mine * P::ROWS + r) * DP + dd) = v;
-          if (dd == 0) x.ml[(int64_t)mine * P::ROWS + r] = make_float2(mm, ll);
-        }
+      }
+      if (i + 1 < n) {  // the next item's queries arrive while this one is finished
+        const int4 next = sm_meta[warp][at + 1 == S ? 0 : at + 1];
+        load_q(next.x, next.y);
       }
       if (!whole) {
         // the CTAs on this item: those whose runs meet its tiles
-        const long long ub = u0 + i - meta.z, ue = ub + meta.w - 1;
-        const int c0 = pa_owner(ub, W, G), c1 = pa_owner(ue, W, G);
-        __threadfence();
+        const long long ub = u0 + i - meta.z;
+        const int c0 = split.owner(ub), c1 = split.owner(ub + meta.w - 1);
         __syncthreads();
-        if (tid == 0) sm_last = atomicAdd(x.counters + c0, 1) == c1 - c0;
+        if (tid == 0) {  // released and acquired at once: with the barriers, for every thread of the CTA
+          const int last = atom_add_acq_rel(x.counters + c0, 1) == c1 - c0;
+          if (last) x.counters[c0] = 0;  // ready for the next call
+          sm_last = last;
+        }
         __syncthreads();
         if (sm_last) {
-          __threadfence();
-          if (tid == 0) x.counters[c0] = 0;  // ready for the next call
-          for (int e = tid; e < rows * quads; e += PA_WARPS * 32) {
-            const int r = e / quads, dd = (e - r * quads) * 4;
+          // each thread adds up four elements over all parts in the order of the runs, FLY parts in flight
+          constexpr int FLY = P::FLY;
+          const int parts = c1 - c0 + 1;
+          for (int e0 = warp * 32; e0 < rows * quads; e0 += PA_WARPS * 32) {
+            const int e = min(e0 + lane, rows * quads - 1), r = e / quads, dd = (e - r * quads) * 4;
             float mm = -INFINITY, ll = 0.f;
-#pragma unroll 8
-            for (int k = c0; k <= c1; ++k)
-              mm = fmaxf(mm, __ldcg(&x.ml[(2 * (int64_t)k + (k == c0)) * P::ROWS + r].x));
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int k = c0; k <= c1; ++k) {
-              const int64_t row = (2 * (int64_t)k + (k == c0)) * P::ROWS + r;
-              const float2 ml = __ldcg(x.ml + row);
-              const float f = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - mm);
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(x.partial + row * DP + dd));
-              v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
-              ll = fmaf(f, ml.y, ll);
+            const float2* ml = x.ml + (int64_t)(2 * c0) * P::ROWS + r;
+            const float* part = x.partial + ((int64_t)(2 * c0) * P::ROWS + r) * DP + dd;
+            for (int k = 0; k < parts; k += FLY) {
+              float2 m8[FLY];
+              float4 y8[FLY];
+#pragma unroll
+              for (int j = 0; j < FLY; ++j) {
+                const int kk = min(k + j, parts - 1);
+                const int64_t row = (int64_t)(2 * kk + (kk == 0)) * P::ROWS;
+                m8[j] = __ldcg(ml + row);
+                y8[j] = __ldcg(reinterpret_cast<const float4*>(part + row * DP));
+              }
+              float top = mm;
+#pragma unroll
+              for (int j = 0; j < FLY; ++j) top = fmaxf(top, m8[j].x);
+              const float keep = mm == -INFINITY ? 0.f : ex2_fast(mm - top);
+              v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+              ll *= keep;
+              mm = top;
+#pragma unroll
+              for (int j = 0; j < FLY; ++j) {
+                if (k + j >= parts) continue;
+                const float f = m8[j].x == -INFINITY ? 0.f : ex2_fast(m8[j].x - mm);
+                v.x = fmaf(f, y8[j].x, v.x); v.y = fmaf(f, y8[j].y, v.y); v.z = fmaf(f, y8[j].z, v.z); v.w = fmaf(f, y8[j].w, v.w);
+                ll = fmaf(f, m8[j].y, ll);
+              }
             }
-            const float inv = ll == 0.f ? 0.f : 1.f / ll;
-            T* o = reinterpret_cast<T*>(p.o) + b * p.o_row + (h0 + r) * p.o_head + dd;
-            pa_store4(o, v, inv, x.o_quads);
-            if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+            if (e0 + lane < rows * quads) finish(r, dd, v, mm, ll);
           }
         }
       }
       __syncthreads();
+      acc.reset();
+      begin = 0;
     }
     at = at + 1 == S ? 0 : at + 1;
     put = put + 1 == S ? 0 : put + 1;
@@ -653,14 +753,15 @@ static auto pa_dispatch(int dtype, int head_dim, int group, F&& f) {
   auto two = [&](auto tag) {
     using T = decltype(tag);
     if (head_dim <= 64) {
-      if (group <= 8) return f(PaKind<PaMma<T, 64, 1, 32, 3, 2>>{});
-      if (group <= 16) return f(PaKind<PaMma<T, 64, 2, 32, 3, 2>>{});
+      if (group <= 8) return f(PaKind<PaMma<T, 64, 1, 32, 2, 3>>{});
+      if (group <= 16) return f(PaKind<PaMma<T, 64, 2, 32, 2, 3>>{});
       return f(PaKind<PaMma<T, 64, 4, 32, 3, 2>>{});
     }
     if (head_dim <= 128) {
-      if (group <= 8) return f(PaKind<PaMma<T, 128, 1, 16, 3, 2>>{});
-      if (group <= 16) return f(PaKind<PaMma<T, 128, 2, 16, 3, 2>>{});
-      return f(PaKind<PaMma<T, 128, 4, 32, 3, 1>>{});
+      if (group <= 8) return f(PaKind<PaMma<T, 128, 1, 16, 2, 3>>{});
+      if (group <= 16) return f(PaKind<PaMma<T, 128, 2, 16, 2, 3>>{});
+      if (group <= 24) return f(PaKind<PaMma<T, 128, 3, 16, 3, 2>>{});
+      return f(PaKind<PaMma<T, 128, 4, 16, 3, 2>>{});
     }
     if (group <= 8) return f(PaKind<PaMma<T, 256, 1, 16, 3, 1>>{});
     return f(PaKind<PaMma<T, 256, 2, 16, 3, 1>>{});
@@ -668,14 +769,14 @@ static auto pa_dispatch(int dtype, int head_dim, int group, F&& f) {
   if (dtype == TH_BF16) return two(__nv_bfloat16{});
   if (dtype == TH_F16) return two(__half{});
   if (head_dim <= 64) {
-    if (group == 1) return f(PaKind<PaSimt<64, 1, 4, 2>>{});
-    if (group <= 4) return f(PaKind<PaSimt<64, 4, 4, 2>>{});
-    return f(PaKind<PaSimt<64, 8, 4, 2>>{});
+    if (group == 1) return f(PaKind<PaSimt<64, 1, 4, 3>>{});
+    if (group <= 4) return f(PaKind<PaSimt<64, 4, 4, 3>>{});
+    return f(PaKind<PaSimt<64, 8, 4, 3>>{});
   }
   if (head_dim <= 128) {
-    if (group == 1) return f(PaKind<PaSimt<128, 1, 3, 2>>{});
-    if (group <= 4) return f(PaKind<PaSimt<128, 4, 3, 2>>{});
-    return f(PaKind<PaSimt<128, 8, 3, 2>>{});
+    if (group == 1) return f(PaKind<PaSimt<128, 1, 2, 3>>{});
+    if (group <= 4) return f(PaKind<PaSimt<128, 4, 2, 3>>{});
+    return f(PaKind<PaSimt<128, 8, 2, 3>>{});
   }
   if (group == 1) return f(PaKind<PaSimt<256, 1, 3, 1>>{});
   return f(PaKind<PaSimt<256, 4, 3, 1>>{});
@@ -741,6 +842,8 @@ extern "C" int th_paged_attention(const th_paged_attention_args* a, void* stream
   PaPlan x{};
   const int64_t cap = (int64_t)a->table_cols * a->page_size;
   x.capacity = (int)(cap < INT32_MAX - 4096 ? cap : INT32_MAX - 4096);
+  x.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctz(a->page_size) : -1;
+  x.same = a->k_page == a->v_page && a->k_head == a->v_head && a->k_slot == a->v_slot;
   x.q_pairs = reinterpret_cast<uintptr_t>(a->q) % 4 == 0 && a->q_row % 2 == 0 && a->q_head % 2 == 0;
   x.o_quads = reinterpret_cast<uintptr_t>(a->o) % (4 * eb) == 0 && a->o_row % 4 == 0 && a->o_head % 4 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
