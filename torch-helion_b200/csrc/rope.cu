@@ -62,8 +62,8 @@ __device__ __forceinline__ RopeUnit<T> rope_unit(const th_rope_args& p, int64_t 
   return u;
 }
 
-// One warp per (token, head), one element pair per lane: every stride,
-// alignment and rotary width.
+// One warp per (token, head), one element pair per lane: the strides,
+// alignments and rotary widths that the vector kernel does not take.
 template <typename T, bool APPEND>
 __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ th_rope_args p) {
   pdl_wait();
@@ -104,11 +104,205 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const __grid_constant__ t
   }
 }
 
+// 16 bytes of T and their rotation by 32-bit products.
+template <typename T>
+union RopeChunk {
+  uint4 u;
+  T e[16 / sizeof(T)];
+};
+
+// The vector kernel: every row (token, head) is 16-byte chunks.  Lane c of a
+// row's 2^shift lanes holds chunks c and c + step: with half pairs those are
+// the two halves of the same pairs, so a rotation needs no other lane; with
+// interleaved pairs each chunk rotates in itself; values and the part of a
+// head past rotary_dim pass through.  A block takes TOK tokens; the cache
+// slots of its tokens are looked up once, behind the first rows' loads, and
+// each row's loads are issued before the row before it is stored.
+constexpr int ROPE_TOK = 4;
+
+template <typename T, bool APPEND, bool INTER>
+__global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ th_rope_args p, int tok, int shift) {
+  constexpr int EPC = 16 / sizeof(T);
+  using Chunk = RopeChunk<T>;
+  __shared__ int sm_pos[ROPE_TOK], sm_page[ROPE_TOK], sm_slot[ROPE_TOK];
+  pdl_wait();
+  pdl_trigger();
+  const int units = p.hq + p.hkv * (APPEND ? 2 : 1), lanes = 1 << shift, c0 = threadIdx.x & (lanes - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * tok;
+  const int n_tok = (int)min((int64_t)tok, p.tokens - t0), rows = n_tok * units, pass = 256 >> shift;
+  const int chunks = p.head_dim / EPC, turned = p.rotary_dim / EPC, half = turned / 2;  // half: only without INTER
+  // (chunk, partner) of lane c: rotated half pairs first, then what passes through two by two
+  auto pair_of = [&](bool rotate, int c, int& a, int& b) {
+    const int step = INTER || !rotate ? (chunks + 1) / 2 : half;
+    const int rest = chunks - 2 * step;  // > 0 only with half pairs on part of the head
+    if (c < step) {
+      a = c;
+      b = c + step;
+    } else {
+      const int k = c - step, s2 = (rest + 1) / 2;
+      a = k < s2 ? 2 * step + k : chunks;
+      b = k < s2 ? 2 * step + s2 + k : chunks;
+    }
+  };
+  struct Row {
+    Chunk a, b;
+    int ia, ib;
+  };
+  auto load = [&](int r, int c, Row& x) {
+    const int tt = r / units, h = r - tt * units;
+    const int64_t t = t0 + tt;
+    const T* src;
+    bool rotate = true;
+    if (h < p.hq) src = (const T*)p.q + t * p.q_token + h * p.q_head;
+    else if (h < p.hq + p.hkv) src = (const T*)p.k + t * p.k_token + (h - p.hq) * p.k_head;
+    else {
+      src = (const T*)p.v + t * p.v_token + (h - p.hq - p.hkv) * p.v_head;
+      rotate = false;
+    }
+    pair_of(rotate, c, x.ia, x.ib);
+    if (x.ia < chunks) x.a.u = *reinterpret_cast<const uint4*>(src + x.ia * EPC);
+    if (x.ib < chunks) x.b.u = *reinterpret_cast<const uint4*>(src + x.ib * EPC);
+  };
+  auto table4 = [](const float* f, float (&v)[4]) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(f));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  };
+  auto turn_inside = [&](Chunk& x, int i, const float* cs, const float* sn) {
+    float c[EPC / 2], s[EPC / 2];
+    if constexpr (EPC == 8) {
+      table4(cs + i * 4, c);
+      table4(sn + i * 4, s);
+    } else {
+      const float2 cc = __ldg(reinterpret_cast<const float2*>(cs + i * 2)), ss = __ldg(reinterpret_cast<const float2*>(sn + i * 2));
+      c[0] = cc.x; c[1] = cc.y; s[0] = ss.x; s[1] = ss.y;
+    }
+#pragma unroll
+    for (int e = 0; e < EPC / 2; ++e) {
+      const float a = to_f32(x.e[2 * e]), b = to_f32(x.e[2 * e + 1]), sg = p.inverse ? -s[e] : s[e];
+      x.e[2 * e] = from_f32<T>(a * c[e] - b * sg);
+      x.e[2 * e + 1] = from_f32<T>(a * sg + b * c[e]);
+    }
+  };
+  auto finish = [&](int r, Row& x) {
+    const int tt = r / units, h = r - tt * units, pos = sm_pos[tt];
+    const int64_t t = t0 + tt;
+    T *dst, *dst2 = nullptr;
+    bool rotate = true;
+    if (h < p.hq) {
+      dst = (T*)p.q_out + t * p.qo_token + h * p.qo_head;
+    } else if (!APPEND) {
+      dst = (T*)p.k_out + t * p.ko_token + (h - p.hq) * p.ko_head;
+    } else {
+      const int page = sm_page[tt], slot = sm_slot[tt];
+      if (h < p.hq + p.hkv) {
+        dst = page >= 0 ? (T*)p.k_pages + page * p.k_page + (h - p.hq) * p.k_phead + slot * p.k_slot : nullptr;
+        dst2 = p.k_out ? (T*)p.k_out + t * p.ko_token + (h - p.hq) * p.ko_head : nullptr;
+      } else {
+        dst = page >= 0 ? (T*)p.v_pages + page * p.v_page + (h - p.hq - p.hkv) * p.v_phead + slot * p.v_slot : nullptr;
+        rotate = false;
+      }
+    }
+    if (pos < 0) {  // padding: the caller's rows are zero, the cache is left alone (page is -1)
+      x.a.u = x.b.u = make_uint4(0, 0, 0, 0);
+    } else if (rotate) {
+      const float* cs = p.cos + pos * p.ld_cs;
+      const float* sn = p.sin + pos * p.ld_cs;
+      if constexpr (INTER) {
+        if (x.ia < turned) turn_inside(x.a, x.ia, cs, sn);
+        if (x.ib < turned) turn_inside(x.b, x.ib, cs, sn);
+      } else if (x.ia < half) {
+#pragma unroll
+        for (int g = 0; g < EPC; g += 4) {
+          float c[4], s[4];
+          table4(cs + x.ia * EPC + g, c);
+          table4(sn + x.ia * EPC + g, s);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = to_f32(x.a.e[g + e]), b = to_f32(x.b.e[g + e]), sg = p.inverse ? -s[e] : s[e];
+            x.a.e[g + e] = from_f32<T>(a * c[e] - b * sg);
+            x.b.e[g + e] = from_f32<T>(a * sg + b * c[e]);
+          }
+        }
+      }
+    }
+    if (dst) {
+      if (x.ia < chunks) *reinterpret_cast<uint4*>(dst + x.ia * EPC) = x.a.u;
+      if (x.ib < chunks) *reinterpret_cast<uint4*>(dst + x.ib * EPC) = x.b.u;
+    }
+    if (dst2) {
+      if (x.ia < chunks) *reinterpret_cast<uint4*>(dst2 + x.ia * EPC) = x.a.u;
+      if (x.ib < chunks) *reinterpret_cast<uint4*>(dst2 + x.ib * EPC) = x.b.u;
+    }
+  };
+
+  int r = threadIdx.x >> shift;
+  Row cur, next;
+  const bool any = r < rows;
+  if (any) load(r, c0, cur);
+  if (threadIdx.x < n_tok) {
+    const int64_t t = t0 + threadIdx.x;
+    int pos = p.positions[t], page = -1, slot = 0;
+    if (pos >= p.table_rows) {
+      atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
+      pos = -1;
+    }
+    if (APPEND && !rope_slot(p, t, pos, page, slot)) page = -1;
+    sm_pos[threadIdx.x] = pos;
+    sm_page[threadIdx.x] = page;
+    sm_slot[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  if (!any) return;
+  // rows, and for heads of more than 2 lanes chunks the rest of each row
+  const int most = (chunks + 1) / 2;  // lanes that a row keeps busy
+  for (int c = c0;;) {
+    int r2 = r + pass, c2 = c;
+    if (r2 >= rows) {
+      r2 = threadIdx.x >> shift;
+      c2 = c + lanes;
+    }
+    const bool more = c2 < most;
+    if (more) load(r2, c2, next);
+    finish(r, cur);
+    if (!more) break;
+    cur = next;
+    r = r2;
+    c = c2;
+  }
+}
+
+// Whether every row of a view starts on 16 bytes.
+static bool rope_rows16(const void* ptr, int eb, int64_t a, int64_t b, int64_t c = 0) {
+  return aligned16(ptr) && a * eb % 16 == 0 && b * eb % 16 == 0 && c * eb % 16 == 0;
+}
+
+static bool rope_vectors(const th_rope_args* a, bool append) {
+  const int eb = elem_bytes(a->dtype), epc = 16 / eb;
+  if (a->head_dim % epc || a->rotary_dim % (a->interleaved ? epc : 2 * epc)) return false;
+  if (!aligned16(a->cos) || !aligned16(a->sin) || a->ld_cs % 4) return false;
+  if (a->hq && (!rope_rows16(a->q, eb, a->q_token, a->q_head) || !rope_rows16(a->q_out, eb, a->qo_token, a->qo_head))) return false;
+  if (a->hkv && (!rope_rows16(a->k, eb, a->k_token, a->k_head) || (a->k_out && !rope_rows16(a->k_out, eb, a->ko_token, a->ko_head))))
+    return false;
+  return !append || (rope_rows16(a->v, eb, a->v_token, a->v_head) && rope_rows16(a->k_pages, eb, a->k_page, a->k_phead, a->k_slot) &&
+                     rope_rows16(a->v_pages, eb, a->v_page, a->v_phead, a->v_slot));
+}
+
 template <typename T, bool APPEND>
 static int rope_launch(const th_rope_args* a, cudaStream_t st, const char* what) {
-  const int64_t warps = a->tokens * (a->hq + a->hkv * (APPEND ? 2 : 1));
-  const int64_t want = (warps + 7) / 8, cap = (int64_t)sm_count() * 64;
-  launch_pdl(rope_any_kernel<T, APPEND>, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, st, *a);
+  const int units = a->hq + a->hkv * (APPEND ? 2 : 1);
+  if (rope_vectors(a, APPEND)) {
+    const int busy = (a->head_dim / (16 / (int)sizeof(T)) + 1) / 2;  // lanes that a row keeps busy
+    int shift = 0;
+    while (shift < 5 && (1 << shift) < busy) ++shift;
+    const int tok = a->tokens >= 4 * 2 * (int64_t)sm_count() ? ROPE_TOK : 1;
+    const int64_t blocks = (a->tokens + tok - 1) / tok;
+    if (blocks > INT32_MAX) return fail(TH_EUNSUPPORTED, "%s: too many tokens", what);
+    auto k = a->interleaved ? rope_vec_kernel<T, APPEND, true> : rope_vec_kernel<T, APPEND, false>;
+    launch_pdl(k, dim3((unsigned)blocks), dim3(256), 0, st, *a, tok, shift);
+  } else {
+    const int64_t want = (a->tokens * units + 7) / 8, cap = (int64_t)sm_count() * 64;
+    launch_pdl(rope_any_kernel<T, APPEND>, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, st, *a);
+  }
   return check_launch(what);
 }
 
