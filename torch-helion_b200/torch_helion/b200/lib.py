@@ -399,6 +399,24 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torc
 
 
 # ------------------------------------------------------- cached decoding
+# One step of a small batch runs these calls in a few microseconds each, so the
+# wrappers check with as few Python-level calls as they can.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _on_device(what: str, first: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """The current stream of the tensors' device, which has to be the current one and the same for all."""
+    dev = first.get_device()
+    if dev < 0:
+        raise B200KernelError(f"{what}: all tensors must live on a CUDA device")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise B200KernelError(f"{what}: all tensors must live on {first.device}, got one on {t.device}")
+    if dev != torch.cuda.current_device():
+        raise B200KernelError(f"{what}: the tensors live on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
 def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
     """(token stride, head stride) of a [tokens, heads, head_dim] view with unit element stride."""
     st = t.stride()
@@ -418,42 +436,39 @@ def _pool(t: torch.Tensor, what: str) -> tuple[int, int, int]:
 
 
 def _ints(t: torch.Tensor, n: int, what: str) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         raise B200KernelError(f"{what} must be contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _page_table(table: torch.Tensor, what: str) -> tuple[int, int, int]:
     """(rows, columns, leading dimension) of an int32 page table."""
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    st = table.stride()
+    if table.dtype != torch.int32 or len(st) != 2 or (st[1] != 1 and table.shape[1] > 1):
         raise B200KernelError(f"{what} must be int32 [sequences, columns] with unit column stride, got {table.dtype} "
                               f"{tuple(table.shape)}")
-    return table.shape[0], table.shape[1], table.stride(0)
+    rows, cols = table.shape
+    return rows, cols, st[0]
 
 
-def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    dev = first.device
-    if dev.type != "cuda":
-        raise B200KernelError("all tensors must live on a CUDA device")
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise B200KernelError(f"all tensors must live on {dev}, got one on {t.device}")
+def _output(out: torch.Tensor | None, like: torch.Tensor, what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise B200KernelError(f"{what} must have the input's shape {tuple(like.shape)} and dtype {like.dtype}")
+    return out
 
 
-def _rope_args(what: str, x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-               interleaved: bool) -> RopeArgs:
-    a = RopeArgs()
-    tokens, _, d = x.shape
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-            or cos.stride() != sin.stride() or (cos.shape[1] > 1 and cos.stride(1) != 1)):
+def _rope_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, d: int) -> tuple[int, int, int]:
+    """(rows, leading dimension, rotary_dim) of the cos and sin tables."""
+    shape, st = cos.shape, cos.stride()
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(st) != 2 or shape != sin.shape
+            or st != sin.stride() or (st[1] != 1 and shape[1] > 1)):
         raise B200KernelError(f"{what}: cos and sin must be fp32 [positions, rotary_dim / 2] of one layout")
-    rotary = 2 * cos.shape[1]
-    if rotary > d:
-        raise B200KernelError(f"{what}: the tables rotate {rotary} elements of heads of {d}")
-    a.positions = _ints(positions, tokens, f"{what}: positions")
-    a.cos, a.sin, a.ld_cs, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
-    a.tokens, a.head_dim, a.rotary_dim, a.interleaved, a.dtype = tokens, d, rotary, int(interleaved), _dt(x)
-    return a
+    rows, half = shape
+    if 2 * half > d:
+        raise B200KernelError(f"{what}: the tables rotate {2 * half} elements of heads of {d}")
+    return rows, st[0], 2 * half
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
@@ -467,29 +482,29 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: 
     turns back: the gradient with respect to the input is ``rope(grad, ..., inverse=True)``.  An output
     may be its input.  A negative position marks padding (zeros); one beyond the tables sets the device
     error word.  Returns ``(q_out, k_out)``."""
-    _same_device(q, k, positions, cos, sin, q_out, k_out)
+    stream = _on_device("rope", q, k, positions, cos, sin, q_out, k_out)
     q_tok, q_head = _heads(q, "rope: q")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif q_out.shape != q.shape or q_out.dtype != q.dtype:
-        raise B200KernelError("rope: q_out must have q's shape and dtype")
-    a = _rope_args("rope", q, positions, cos, sin, interleaved)
-    a.q, a.q_token, a.q_head, a.hq = q.data_ptr(), q_tok, q_head, q.shape[1]
-    a.q_out, (a.qo_token, a.qo_head) = q_out.data_ptr(), _heads(q_out, "rope: q_out")
+    tokens, hq, d = q.shape
+    rows, ld, rotary = _rope_tables("rope", cos, sin, d)
+    q_out = _output(q_out, q, "rope: q_out")
+    qo_tok, qo_head = _heads(q_out, "rope: q_out")
+    dtype = _dt(q)
+    k_args = (None, 0, 0, None, 0, 0)
+    hkv = 0
     if k is not None:
-        if k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        k_tok, k_head = _heads(k, "rope: k")
+        k_tokens, hkv, dk = k.shape
+        if k.dtype != q.dtype or k_tokens != tokens or dk != d:
             raise B200KernelError("rope: k must be [tokens, heads, head_dim] like q, of q's dtype")
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        elif k_out.shape != k.shape or k_out.dtype != k.dtype:
-            raise B200KernelError("rope: k_out must have k's shape and dtype")
-        a.k, (a.k_token, a.k_head), a.hkv = k.data_ptr(), _heads(k, "rope: k"), k.shape[1]
-        a.k_out, (a.ko_token, a.ko_head) = k_out.data_ptr(), _heads(k_out, "rope: k_out")
+        k_out = _output(k_out, k, "rope: k_out")
+        k_args = (k.data_ptr(), k_tok, k_head, k_out.data_ptr(), *_heads(k_out, "rope: k_out"))
     elif k_out is not None:
         raise B200KernelError("rope: k_out without k")
-    a.inverse = int(inverse)
-    if a.tokens:
-        _check(load().th_rope(ctypes.byref(a), _stream()), "th_rope")
+    at = _ints(positions, tokens, "rope: positions")
+    if tokens:
+        a = RopeArgs(q.data_ptr(), q_tok, q_head, q_out.data_ptr(), qo_tok, qo_head, *k_args, at, cos.data_ptr(),
+                     sin.data_ptr(), ld, tokens, rows, hq, hkv, d, rotary, bool(interleaved), bool(inverse), dtype)
+        _check(load().th_rope(ctypes.byref(a), stream), "th_rope")
     return q_out, k_out
 
 
@@ -504,41 +519,41 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     pools [num_pages, hkv, page_size, d] (any page, head and slot strides).  A negative position marks
     padding: nothing is stored and its q_out row is zero.  Ids out of range set the device error word.
     ``k_out`` (optional, like k) receives the rotated keys as well.  Returns ``q_out`` (None without q)."""
-    _same_device(k, q, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out)
-    a = _rope_args("rope_append", k, positions, cos, sin, interleaved)
-    tokens, hkv, d = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
+    stream = _on_device("rope_append", k, q, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out)
+    k_tok, k_head = _heads(k, "rope_append: k")
+    tokens, hkv, d = shape = k.shape
+    dt = k.dtype
+    if v.shape != shape or v.dtype != dt:
         raise B200KernelError("rope_append: v must have k's shape and dtype")
-    for pool in (k_pages, v_pages):
-        if pool.dtype != k.dtype or pool.dim() != 4 or pool.shape != k_pages.shape or pool.shape[1] != hkv or pool.shape[3] != d:
-            raise B200KernelError("rope_append: the pools must be [num_pages, hkv, page_size, d] of k's dtype")
+    rows, ld, rotary = _rope_tables("rope_append", cos, sin, d)
+    kp, vp, pool = _pool(k_pages, "rope_append: k_pages"), _pool(v_pages, "rope_append: v_pages"), k_pages.shape
+    if k_pages.dtype != dt or v_pages.dtype != dt or v_pages.shape != pool or pool[1] != hkv or pool[3] != d:
+        raise B200KernelError("rope_append: the pools must be [num_pages, hkv, page_size, d] of k's dtype")
+    q_args = (None, 0, 0, None, 0, 0)
+    hq = 0
     if q is not None:
-        if q.dtype != k.dtype or q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != d:
+        q_tok, q_head = _heads(q, "rope_append: q")
+        q_tokens, hq, dq = q.shape
+        if q.dtype != dt or q_tokens != tokens or dq != d:
             raise B200KernelError("rope_append: q must be [tokens, heads, head_dim] like k, of k's dtype")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
-            raise B200KernelError("rope_append: q_out must have q's shape and dtype")
-        a.q, (a.q_token, a.q_head), a.hq = q.data_ptr(), _heads(q, "rope_append: q"), q.shape[1]
-        a.q_out, (a.qo_token, a.qo_head) = q_out.data_ptr(), _heads(q_out, "rope_append: q_out")
+        q_out = _output(q_out, q, "rope_append: q_out")
+        q_args = (q.data_ptr(), q_tok, q_head, q_out.data_ptr(), *_heads(q_out, "rope_append: q_out"))
     elif q_out is not None:
         raise B200KernelError("rope_append: q_out without q")
-    a.k, (a.k_token, a.k_head), a.hkv = k.data_ptr(), _heads(k, "rope_append: k"), hkv
+    ko_args = (None, 0, 0)
     if k_out is not None:
-        if k_out.shape != k.shape or k_out.dtype != k.dtype:
-            raise B200KernelError("rope_append: k_out must have k's shape and dtype")
-        a.k_out, (a.ko_token, a.ko_head) = k_out.data_ptr(), _heads(k_out, "rope_append: k_out")
-    a.v, (a.v_token, a.v_head) = v.data_ptr(), _heads(v, "rope_append: v")
-    a.k_pages, (a.k_page, a.k_phead, a.k_slot) = k_pages.data_ptr(), _pool(k_pages, "rope_append: k_pages")
-    a.v_pages, (a.v_page, a.v_phead, a.v_slot) = v_pages.data_ptr(), _pool(v_pages, "rope_append: v_pages")
-    a.table, (a.batch, a.table_cols, a.ld_table) = table.data_ptr(), _page_table(table, "rope_append: table")
-    a.num_pages, a.page_size = k_pages.shape[0], k_pages.shape[2]
-    if seqs is not None:
-        a.seqs = _ints(seqs, tokens, "rope_append: seqs")
-    elif a.batch < tokens:
-        raise B200KernelError(f"rope_append: {tokens} tokens without seqs need as many rows of table, got {a.batch}")
+        ko_args = (_output(k_out, k, "rope_append: k_out").data_ptr(), *_heads(k_out, "rope_append: k_out"))
+    batch, cols, ld_table = _page_table(table, "rope_append: table")
+    if seqs is None and batch < tokens:
+        raise B200KernelError(f"rope_append: {tokens} tokens without seqs need as many rows of table, got {batch}")
+    at = _ints(positions, tokens, "rope_append: positions")
+    of = None if seqs is None else _ints(seqs, tokens, "rope_append: seqs")
     if tokens:
-        _check(load().th_rope_append(ctypes.byref(a), _stream()), "th_rope_append")
+        a = RopeArgs(*q_args, k.data_ptr(), k_tok, k_head, *ko_args, at, cos.data_ptr(), sin.data_ptr(), ld, tokens, rows,
+                     hq, hkv, d, rotary, bool(interleaved), 0, _dt(k), v.data_ptr(), *_heads(v, "rope_append: v"),
+                     k_pages.data_ptr(), *kp, v_pages.data_ptr(), *vp, table.data_ptr(), ld_table, of, batch, cols,
+                     pool[2], pool[0])
+        _check(load().th_rope_append(ctypes.byref(a), stream), "th_rope_append")
     return q_out
 
 
@@ -563,39 +578,31 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (fp32 [batch, hq], optional) receives log sum exp of the scores.  ``workspace`` comes from
     :func:`paged_attention_workspace` and may be kept; calls that share one must be ordered on the GPU
     (None: a fresh one per call)."""
-    _same_device(q, k_pages, v_pages, table, lens, out, lse, workspace)
+    stream = _on_device("paged_attention", q, k_pages, v_pages, table, lens, out, lse, workspace)
     q_row, q_head = _heads(q, "paged_attention: q")
     batch, hq, d = q.shape
-    pool = _pool(k_pages, "paged_attention: k_pages")
-    num_pages, hkv, page_size, dk = k_pages.shape
-    if v_pages.shape != k_pages.shape or dk != d or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+    dt = q.dtype
+    kp, vp, pool = _pool(k_pages, "paged_attention: k_pages"), _pool(v_pages, "paged_attention: v_pages"), k_pages.shape
+    num_pages, hkv, page_size, dk = pool
+    if v_pages.shape != pool or dk != d or k_pages.dtype != dt or v_pages.dtype != dt:
         raise B200KernelError("paged_attention: the pools must be [num_pages, hkv, page_size, d] of q's dtype and head size")
     rows, cols, ld = _page_table(table, "paged_attention: table")
     if rows < batch:
         raise B200KernelError(f"paged_attention: {batch} queries need as many rows of table, got {rows}")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise B200KernelError("paged_attention: out must have q's shape and dtype")
+    out = _output(out, q, "paged_attention: out")
+    o_row, o_head = _heads(out, "paged_attention: out")
+    n = _ints(lens, batch, "paged_attention: lens")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous()):
+        raise B200KernelError("paged_attention: lse must be contiguous fp32 [batch, hq]")
     if batch == 0:
         return out
     if workspace is None:
         workspace = paged_attention_workspace(q, k_pages)
-    a = PagedAttentionArgs()
-    a.q, a.q_row, a.q_head = q.data_ptr(), q_row, q_head
-    a.o, (a.o_row, a.o_head) = out.data_ptr(), _heads(out, "paged_attention: out")
-    if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous():
-            raise B200KernelError("paged_attention: lse must be contiguous fp32 [batch, hq]")
-        a.lse = lse.data_ptr()
-    a.k_pages, (a.k_page, a.k_head, a.k_slot) = k_pages.data_ptr(), pool
-    a.v_pages, (a.v_page, a.v_head, a.v_slot) = v_pages.data_ptr(), _pool(v_pages, "paged_attention: v_pages")
-    a.table, a.ld_table, a.lens = table.data_ptr(), ld, _ints(lens, batch, "paged_attention: lens")
-    a.batch, a.hq, a.hkv, a.head_dim, a.page_size, a.num_pages, a.table_cols = batch, hq, hkv, d, page_size, num_pages, cols
-    a.window, a.softcap, a.dtype = window, softcap, _dt(q)
-    a.scale = d ** -0.5 if scale is None else scale
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _check(load().th_paged_attention(ctypes.byref(a), _stream()), "th_paged_attention")
+    a = PagedAttentionArgs(q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head, None if lse is None else lse.data_ptr(),
+                           k_pages.data_ptr(), *kp, v_pages.data_ptr(), *vp, table.data_ptr(), ld, n, batch, hq, hkv, d,
+                           page_size, num_pages, cols, window, d ** -0.5 if scale is None else scale, softcap, _dt(q),
+                           workspace.data_ptr(), workspace.nbytes)
+    _check(load().th_paged_attention(ctypes.byref(a), stream), "th_paged_attention")
     return out
 
 
@@ -606,15 +613,16 @@ def page_copy(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, counts:
     plane that shares the page ids: layers x keys and values x heads), ``src``, ``dst`` and ``counts``
     int32 [pairs] (counts None: whole pages).  A negative id skips the pair.  Destinations must be
     distinct and none may be a source; ids out of range set the device error word."""
-    _same_device(pages, src, dst, counts)
-    if pages.dim() != 4 or pages.stride(3) != 1 or (pages.shape[2] > 1 and pages.stride(2) != pages.shape[3]):
+    stream = _on_device("page_copy", pages, src, dst, counts)
+    shape, st = pages.shape, pages.stride()
+    if len(st) != 4 or st[3] != 1 or (st[2] != shape[3] and shape[2] > 1):
         raise B200KernelError("page_copy: pages must be [num_pages, planes, page_size, width] with contiguous slots, got "
-                              f"shape {tuple(pages.shape)} stride {pages.stride()}")
-    n, es = src.shape[0] if src.dim() == 1 else -1, pages.element_size()
+                              f"shape {tuple(shape)} stride {st}")
+    if src.dim() != 1:
+        raise B200KernelError("page_copy: src must be one-dimensional")
+    n, es = src.shape[0], pages.element_size()
+    ids = _ints(src, n, "page_copy: src"), _ints(dst, n, "page_copy: dst"), None if counts is None else _ints(counts, n, "page_copy: counts")
     if n == 0 or pages.numel() == 0:
         return
-    a = PageCopyArgs(pages.data_ptr(), pages.stride(0) * es, pages.stride(1) * es, pages.shape[3] * es,
-                     _ints(src, n, "page_copy: src"), _ints(dst, n, "page_copy: dst"),
-                     None if counts is None else _ints(counts, n, "page_copy: counts"), n, pages.shape[0],
-                     pages.shape[1], pages.shape[2])
-    _check(load().th_page_copy(ctypes.byref(a), _stream()), "th_page_copy")
+    a = PageCopyArgs(pages.data_ptr(), st[0] * es, st[1] * es, shape[3] * es, *ids, n, shape[0], shape[1], shape[2])
+    _check(load().th_page_copy(ctypes.byref(a), stream), "th_page_copy")
