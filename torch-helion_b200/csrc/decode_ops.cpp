@@ -1,0 +1,406 @@
+// Python entry points of the decoding operators (rope, rope_append,
+// paged_attention, page_copy).
+//
+// One decoding step of a small batch takes a few microseconds on the device,
+// less than a ctypes wrapper needs to look at eight tensors.  These functions
+// make the same checks on the tensors themselves, fill the argument structs of
+// th_b200.h and call the library on the current torch stream; about one
+// microsecond a call, the launch beside it.  lib.py documents the arguments
+// and hands over the library's functions and its exception (init).
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <optional>
+
+#include "../../include/th_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+PyObject* g_error = nullptr;
+decltype(&th_rope) g_rope = nullptr;
+decltype(&th_rope_append) g_rope_append = nullptr;
+decltype(&th_paged_attention) g_paged_attention = nullptr;
+decltype(&th_paged_attention_workspace_size) g_workspace_size = nullptr;
+decltype(&th_page_copy) g_page_copy = nullptr;
+decltype(&th_last_error_string) g_last_error = nullptr;
+
+// A refusal; caught at the entry points.
+struct Refused {};
+
+[[noreturn]] void refuse(const char* fmt, ...) {
+  char text[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(text, sizeof(text), fmt, ap);
+  va_end(ap);
+  PyErr_SetString(g_error, text);
+  throw Refused{};
+}
+
+void status(int rc, const char* what) {
+  if (rc != TH_OK) refuse("%s failed with status %d: %s", what, rc, g_last_error());
+}
+
+// What an argument is called in a message.
+struct Name {
+  const char *op, *arg;
+};
+
+const Tensor* tensor_or_none(PyObject* o, Name n) {
+  if (o == Py_None) return nullptr;
+  if (!THPVariable_Check(o)) refuse("%s: %s must be a tensor, got %s", n.op, n.arg, Py_TYPE(o)->tp_name);
+  return &THPVariable_Unpack(o);
+}
+
+const Tensor& tensor(PyObject* o, Name n) {
+  const Tensor* t = tensor_or_none(o, n);
+  if (!t) refuse("%s: %s must be a tensor, got None", n.op, n.arg);
+  return *t;
+}
+
+// The current stream of the tensors' device, which has to be the current
+// device and the same for all.
+template <typename... Ts>
+cudaStream_t stream_of(const char* op, const Tensor& first, const Ts*... rest) {
+  if (!first.is_cuda()) refuse("%s: all tensors must live on a CUDA device", op);
+  const int dev = first.get_device();
+  for (const Tensor* t : {static_cast<const Tensor*>(rest)...})
+    if (t && (!t->is_cuda() || t->get_device() != dev))
+      refuse("%s: all tensors must live on cuda:%d, got one on %s", op, dev, t->device().str().c_str());
+  const int now = c10::cuda::current_device();
+  if (dev != now) refuse("%s: the tensors live on cuda:%d, the current device is cuda:%d", op, dev, now);
+  return c10::cuda::getCurrentCUDAStream(dev).stream();
+}
+
+int code(const char* op, const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return TH_F32;
+    case at::kBFloat16: return TH_BF16;
+    case at::kHalf: return TH_F16;
+    default: refuse("%s: unsupported dtype %s", op, c10::toString(t.scalar_type()));
+  }
+}
+
+// [tokens, heads, head_dim] with unit element stride.
+void heads(const Tensor& t, Name n, int64_t& token, int64_t& head) {
+  if (t.dim() != 3 || (t.stride(2) != 1 && t.size(2) > 1))
+    refuse("%s: %s must be [tokens, heads, head_dim] with unit element stride", n.op, n.arg);
+  token = t.stride(0);
+  head = t.stride(1);
+}
+
+// [num_pages, heads, page_size, head_dim] with unit element stride.
+void pool(const Tensor& t, Name n, int64_t& page, int64_t& head, int64_t& slot) {
+  if (t.dim() != 4 || t.stride(3) != 1)
+    refuse("%s: %s must be [num_pages, heads, page_size, head_dim] with unit element stride", n.op, n.arg);
+  page = t.stride(0);
+  head = t.stride(1);
+  slot = t.stride(2);
+}
+
+const int32_t* ints(const Tensor& t, int64_t size, Name n) {
+  if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != size || (size > 1 && t.stride(0) != 1))
+    refuse("%s: %s must be contiguous int32 [%lld]", n.op, n.arg, (long long)size);
+  return static_cast<const int32_t*>(t.const_data_ptr());
+}
+
+const int32_t* page_table(const Tensor& t, const char* op, int32_t& rows, int32_t& cols, int64_t& ld) {
+  if (t.scalar_type() != at::kInt || t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1))
+    refuse("%s: table must be int32 [sequences, columns] with unit column stride", op);
+  if (t.size(0) > INT32_MAX || t.size(1) > INT32_MAX) refuse("%s: table is too large", op);
+  rows = (int32_t)t.size(0);
+  cols = (int32_t)t.size(1);
+  ld = t.stride(0);
+  return static_cast<const int32_t*>(t.const_data_ptr());
+}
+
+// `out`, or a new contiguous tensor like `like` held in `made`.
+const Tensor& output(const Tensor* out, const Tensor& like, Name n, std::optional<Tensor>& made) {
+  if (!out) {
+    made = at::empty_like(like, at::TensorOptions(), at::MemoryFormat::Contiguous);
+    return *made;
+  }
+  if (out->sizes() != like.sizes() || out->scalar_type() != like.scalar_type())
+    refuse("%s: %s must have the input's shape and dtype", n.op, n.arg);
+  return *out;
+}
+
+PyObject* give(PyObject* given, std::optional<Tensor>& made) {
+  if (made) return THPVariable_Wrap(std::move(*made));
+  Py_INCREF(given);
+  return given;
+}
+
+void rotary(const char* op, const Tensor& cos, const Tensor& sin, th_rope_args& a) {
+  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.sizes() != sin.sizes() ||
+      cos.strides() != sin.strides() || (cos.size(1) > 1 && cos.stride(1) != 1) || cos.size(0) > INT32_MAX)
+    refuse("%s: cos and sin must be fp32 [positions, rotary_dim / 2] of one layout", op);
+  if (2 * cos.size(1) > a.head_dim)
+    refuse("%s: the tables rotate %lld elements of heads of %d", op, (long long)(2 * cos.size(1)), a.head_dim);
+  a.cos = static_cast<const float*>(cos.const_data_ptr());
+  a.sin = static_cast<const float*>(sin.const_data_ptr());
+  a.ld_cs = cos.stride(0);
+  a.table_rows = (int32_t)cos.size(0);
+  a.rotary_dim = (int32_t)(2 * cos.size(1));
+}
+
+void like_k(const char* op, const Tensor& t, const char* arg, const Tensor& k) {
+  if (t.dim() != 3 || t.scalar_type() != k.scalar_type() || t.size(0) != k.size(0) || t.size(2) != k.size(2))
+    refuse("%s: %s must be [tokens, heads, head_dim] with the other heads' tokens, head_dim and dtype", op, arg);
+}
+
+int truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Refused{};
+  return v;
+}
+
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused{};
+  return v;
+}
+
+// (q, k, positions, cos, sin, q_out, k_out, interleaved, inverse)
+PyObject* rope(PyObject* const* v) {
+  const char* op = "rope";
+  const Tensor &q = tensor(v[0], {op, "q"}), &pos = tensor(v[2], {op, "positions"}), &cos = tensor(v[3], {op, "cos"}),
+               &sin = tensor(v[4], {op, "sin"});
+  const Tensor *k = tensor_or_none(v[1], {op, "k"}), *q_out = tensor_or_none(v[5], {op, "q_out"}),
+               *k_out = tensor_or_none(v[6], {op, "k_out"});
+  const cudaStream_t st = stream_of(op, q, k, &pos, &cos, &sin, q_out, k_out);
+  th_rope_args a{};
+  heads(q, {op, "q"}, a.q_token, a.q_head);
+  a.q = q.const_data_ptr();
+  a.tokens = q.size(0);
+  a.hq = (int32_t)q.size(1);
+  a.head_dim = (int32_t)q.size(2);
+  a.dtype = code(op, q);
+  rotary(op, cos, sin, a);
+  std::optional<Tensor> made_q, made_k;
+  const Tensor& qo = output(q_out, q, {op, "q_out"}, made_q);
+  heads(qo, {op, "q_out"}, a.qo_token, a.qo_head);
+  a.q_out = qo.data_ptr();
+  if (k) {
+    like_k(op, *k, "k", q);
+    heads(*k, {op, "k"}, a.k_token, a.k_head);
+    a.k = k->const_data_ptr();
+    a.hkv = (int32_t)k->size(1);
+    const Tensor& ko = output(k_out, *k, {op, "k_out"}, made_k);
+    heads(ko, {op, "k_out"}, a.ko_token, a.ko_head);
+    a.k_out = ko.data_ptr();
+  } else if (k_out) {
+    refuse("rope: k_out without k");
+  }
+  a.positions = ints(pos, a.tokens, {op, "positions"});
+  a.interleaved = truth(v[7]);
+  a.inverse = truth(v[8]);
+  if (a.tokens) status(g_rope(&a, st), "th_rope");
+  PyObject *first = give(v[5], made_q), *second = give(k ? v[6] : Py_None, made_k);
+  return first && second ? Py_BuildValue("(NN)", first, second) : nullptr;
+}
+
+// (q, k, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out, interleaved)
+PyObject* rope_append(PyObject* const* o) {
+  const char* op = "rope_append";
+  const Tensor *q = tensor_or_none(o[0], {op, "q"}), *seqs = tensor_or_none(o[9], {op, "seqs"}),
+               *q_out = tensor_or_none(o[10], {op, "q_out"}), *k_out = tensor_or_none(o[11], {op, "k_out"});
+  const Tensor &k = tensor(o[1], {op, "k"}), &v = tensor(o[2], {op, "v"}), &pos = tensor(o[3], {op, "positions"}),
+               &cos = tensor(o[4], {op, "cos"}), &sin = tensor(o[5], {op, "sin"}), &kp = tensor(o[6], {op, "k_pages"}),
+               &vp = tensor(o[7], {op, "v_pages"}), &table = tensor(o[8], {op, "table"});
+  const cudaStream_t st = stream_of(op, k, q, &v, &pos, &cos, &sin, &kp, &vp, &table, seqs, q_out, k_out);
+  th_rope_args a{};
+  heads(k, {op, "k"}, a.k_token, a.k_head);
+  a.k = k.const_data_ptr();
+  a.tokens = k.size(0);
+  a.hkv = (int32_t)k.size(1);
+  a.head_dim = (int32_t)k.size(2);
+  a.dtype = code(op, k);
+  rotary(op, cos, sin, a);
+  if (v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type()) refuse("rope_append: v must have k's shape and dtype");
+  heads(v, {op, "v"}, a.v_token, a.v_head);
+  a.v = v.const_data_ptr();
+  pool(kp, {op, "k_pages"}, a.k_page, a.k_phead, a.k_slot);
+  pool(vp, {op, "v_pages"}, a.v_page, a.v_phead, a.v_slot);
+  if (kp.scalar_type() != k.scalar_type() || vp.scalar_type() != k.scalar_type() || kp.sizes() != vp.sizes() ||
+      kp.size(1) != k.size(1) || kp.size(3) != k.size(2) || kp.size(0) > INT32_MAX || kp.size(2) > INT32_MAX)
+    refuse("rope_append: the pools must be [num_pages, hkv, page_size, d] of k's dtype");
+  a.k_pages = kp.data_ptr();
+  a.v_pages = vp.data_ptr();
+  a.num_pages = (int32_t)kp.size(0);
+  a.page_size = (int32_t)kp.size(2);
+  a.table = page_table(table, op, a.batch, a.table_cols, a.ld_table);
+  std::optional<Tensor> made;
+  if (q) {
+    like_k(op, *q, "q", k);
+    heads(*q, {op, "q"}, a.q_token, a.q_head);
+    a.q = q->const_data_ptr();
+    a.hq = (int32_t)q->size(1);
+    const Tensor& qo = output(q_out, *q, {op, "q_out"}, made);
+    heads(qo, {op, "q_out"}, a.qo_token, a.qo_head);
+    a.q_out = qo.data_ptr();
+  } else if (q_out) {
+    refuse("rope_append: q_out without q");
+  }
+  if (k_out) {
+    std::optional<Tensor> none;
+    const Tensor& ko = output(k_out, k, {op, "k_out"}, none);
+    heads(ko, {op, "k_out"}, a.ko_token, a.ko_head);
+    a.k_out = ko.data_ptr();
+  }
+  a.positions = ints(pos, a.tokens, {op, "positions"});
+  if (seqs) a.seqs = ints(*seqs, a.tokens, {op, "seqs"});
+  else if (a.batch < a.tokens)
+    refuse("rope_append: %lld tokens without seqs need as many rows of table, got %d", (long long)a.tokens, a.batch);
+  a.interleaved = truth(o[12]);
+  if (a.tokens) status(g_rope_append(&a, st), "th_rope_append");
+  return give(q ? o[10] : Py_None, made);
+}
+
+// (q, k_pages, v_pages, table, lens, out, scale, softcap, window, lse, workspace)
+PyObject* paged_attention(PyObject* const* o) {
+  const char* op = "paged_attention";
+  const Tensor &q = tensor(o[0], {op, "q"}), &kp = tensor(o[1], {op, "k_pages"}), &vp = tensor(o[2], {op, "v_pages"}),
+               &table = tensor(o[3], {op, "table"}), &lens = tensor(o[4], {op, "lens"});
+  const Tensor *out = tensor_or_none(o[5], {op, "out"}), *lse = tensor_or_none(o[9], {op, "lse"}),
+               *ws = tensor_or_none(o[10], {op, "workspace"});
+  const cudaStream_t st = stream_of(op, q, &kp, &vp, &table, &lens, out, lse, ws);
+  th_paged_attention_args a{};
+  heads(q, {op, "q"}, a.q_row, a.q_head);
+  a.q = q.const_data_ptr();
+  a.dtype = code(op, q);
+  pool(kp, {op, "k_pages"}, a.k_page, a.k_head, a.k_slot);
+  pool(vp, {op, "v_pages"}, a.v_page, a.v_head, a.v_slot);
+  if (kp.sizes() != vp.sizes() || kp.size(3) != q.size(2) || kp.scalar_type() != q.scalar_type() ||
+      vp.scalar_type() != q.scalar_type() || kp.size(0) > INT32_MAX || kp.size(1) > INT32_MAX || kp.size(2) > INT32_MAX ||
+      q.size(0) > INT32_MAX || q.size(1) > INT32_MAX || q.size(2) > INT32_MAX)
+    refuse("paged_attention: the pools must be [num_pages, hkv, page_size, d] of q's dtype and head size");
+  a.k_pages = kp.const_data_ptr();
+  a.v_pages = vp.const_data_ptr();
+  a.batch = (int32_t)q.size(0);
+  a.hq = (int32_t)q.size(1);
+  a.head_dim = (int32_t)q.size(2);
+  a.num_pages = (int32_t)kp.size(0);
+  a.hkv = (int32_t)kp.size(1);
+  a.page_size = (int32_t)kp.size(2);
+  int32_t rows;
+  a.table = page_table(table, op, rows, a.table_cols, a.ld_table);
+  if (rows < a.batch) refuse("paged_attention: %d queries need as many rows of table, got %d", a.batch, rows);
+  std::optional<Tensor> made, own_ws;
+  const Tensor& result = output(out, q, {op, "out"}, made);
+  heads(result, {op, "out"}, a.o_row, a.o_head);
+  a.o = result.data_ptr();
+  a.lens = ints(lens, a.batch, {op, "lens"});
+  if (lse) {
+    if (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != a.batch || lse->size(1) != a.hq || !lse->is_contiguous())
+      refuse("paged_attention: lse must be contiguous fp32 [batch, hq]");
+    a.lse = static_cast<float*>(lse->data_ptr());
+  }
+  a.scale = o[6] == Py_None ? (float)(1.0 / std::sqrt((double)a.head_dim)) : (float)number(o[6]);
+  a.softcap = (float)number(o[7]);
+  const long window = PyLong_AsLong(o[8]);
+  if (window == -1 && PyErr_Occurred()) throw Refused{};
+  if (window < 0) refuse("paged_attention: window must not be negative");
+  a.window = (int32_t)std::min<long>(window, INT32_MAX);  // beyond any length: no window
+  if (a.batch) {
+    if (!ws) {
+      const size_t need = g_workspace_size(a.hq, a.hkv, a.head_dim, a.dtype);
+      if (need == 0) refuse("paged_attention: heads %d over %d of %d are not supported", a.hq, a.hkv, a.head_dim);
+      own_ws = at::zeros({(int64_t)need}, q.options().dtype(at::kByte));
+      ws = &*own_ws;
+    }
+    a.workspace = ws->data_ptr();
+    a.workspace_bytes = ws->nbytes();
+    status(g_paged_attention(&a, st), "th_paged_attention");
+  }
+  return give(o[5], made);
+}
+
+// (pages, src, dst, counts)
+PyObject* page_copy(PyObject* const* o) {
+  const char* op = "page_copy";
+  const Tensor &pages = tensor(o[0], {op, "pages"}), &src = tensor(o[1], {op, "src"}), &dst = tensor(o[2], {op, "dst"});
+  const Tensor* counts = tensor_or_none(o[3], {op, "counts"});
+  const cudaStream_t st = stream_of(op, pages, &src, &dst, counts);
+  if (pages.dim() != 4 || pages.stride(3) != 1 || (pages.size(2) > 1 && pages.stride(2) != pages.size(3)))
+    refuse("page_copy: pages must be [num_pages, planes, page_size, width] with contiguous slots");
+  if (src.dim() != 1) refuse("page_copy: src must be one-dimensional");
+  const int64_t n = src.size(0), es = pages.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (pages.size(i) > INT32_MAX || n > INT32_MAX) refuse("page_copy: a size is beyond 2^31");
+  th_page_copy_args a{};
+  a.src = ints(src, n, {op, "src"});
+  a.dst = ints(dst, n, {op, "dst"});
+  if (counts) a.counts = ints(*counts, n, {op, "counts"});
+  if (n && pages.numel()) {
+    a.pages = pages.data_ptr();
+    a.page_stride = pages.stride(0) * es;
+    a.plane_stride = pages.stride(1) * es;
+    a.slot_bytes = pages.size(3) * es;
+    a.pairs = (int32_t)n;
+    a.num_pages = (int32_t)pages.size(0);
+    a.planes = (int32_t)pages.size(1);
+    a.page_size = (int32_t)pages.size(2);
+    status(g_page_copy(&a, st), "th_page_copy");
+  }
+  Py_RETURN_NONE;
+}
+
+// No C++ exception leaves an entry point.
+template <PyObject* (*F)(PyObject* const*), int N>
+PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != N) return PyErr_Format(PyExc_TypeError, "%d arguments are needed, got %zd", N, n);
+  try {
+    return F(args);
+  } catch (const Refused&) {
+    return nullptr;
+  } catch (const std::exception& e) {
+    PyErr_SetString(g_error, e.what());
+    return nullptr;
+  }
+}
+
+// init(exception, address of th_rope, th_rope_append, th_paged_attention,
+//      th_paged_attention_workspace_size, th_page_copy, th_last_error_string)
+PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) return PyErr_Format(PyExc_TypeError, "init takes 7 arguments");
+  void* f[6];
+  for (int i = 0; i < 6; ++i) {
+    f[i] = PyLong_AsVoidPtr(args[i + 1]);
+    if (!f[i]) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "init: a NULL function");
+  }
+  Py_INCREF(args[0]);
+  Py_XDECREF(g_error);
+  g_error = args[0];
+  g_rope = reinterpret_cast<decltype(g_rope)>(f[0]);
+  g_rope_append = reinterpret_cast<decltype(g_rope_append)>(f[1]);
+  g_paged_attention = reinterpret_cast<decltype(g_paged_attention)>(f[2]);
+  g_workspace_size = reinterpret_cast<decltype(g_workspace_size)>(f[3]);
+  g_page_copy = reinterpret_cast<decltype(g_page_copy)>(f[4]);
+  g_last_error = reinterpret_cast<decltype(g_last_error)>(f[5]);
+  Py_RETURN_NONE;
+}
+
+#define FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {FAST("init", init),
+                         FAST("rope", (entry<rope, 9>)),
+                         FAST("rope_append", (entry<rope_append, 13>)),
+                         FAST("paged_attention", (entry<paged_attention, 11>)),
+                         FAST("page_copy", (entry<page_copy, 4>)),
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "th_decode_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_th_decode_ops() { return PyModule_Create(&module); }

@@ -399,76 +399,30 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor) -> torc
 
 
 # ------------------------------------------------------- cached decoding
-# One step of a small batch runs these calls in a few microseconds each, so the
-# wrappers check with as few Python-level calls as they can.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+# These calls take a few microseconds on the device, so their arguments are
+# checked and handed over by compiled entry points (csrc/decode_ops.cpp).
+_OPS = None
 
 
-def _on_device(what: str, first: torch.Tensor, *ts: torch.Tensor | None) -> int:
-    """The current stream of the tensors' device, which has to be the current one and the same for all."""
-    dev = first.get_device()
-    if dev < 0:
-        raise B200KernelError(f"{what}: all tensors must live on a CUDA device")
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            raise B200KernelError(f"{what}: all tensors must live on {first.device}, got one on {t.device}")
-    if dev != torch.cuda.current_device():
-        raise B200KernelError(f"{what}: the tensors live on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+def _ops():
+    """The compiled entry points, loaded once beside the library."""
+    global _OPS
+    if _OPS is None:
+        from importlib import machinery, util
 
-
-def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
-    """(token stride, head stride) of a [tokens, heads, head_dim] view with unit element stride."""
-    st = t.stride()
-    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
-        raise B200KernelError(f"{what} must be [tokens, heads, head_dim] with unit element stride, got shape "
-                              f"{tuple(t.shape)} stride {st}")
-    return st[0], st[1]
-
-
-def _pool(t: torch.Tensor, what: str) -> tuple[int, int, int]:
-    """(page, head, slot) strides of a page pool [num_pages, heads, page_size, head_dim]."""
-    st = t.stride()
-    if len(st) != 4 or st[3] != 1:
-        raise B200KernelError(f"{what} must be [num_pages, heads, page_size, head_dim] with unit element stride, got "
-                              f"shape {tuple(t.shape)} stride {st}")
-    return st[0], st[1], st[2]
-
-
-def _ints(t: torch.Tensor, n: int, what: str) -> int:
-    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
-        raise B200KernelError(f"{what} must be contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
-
-
-def _page_table(table: torch.Tensor, what: str) -> tuple[int, int, int]:
-    """(rows, columns, leading dimension) of an int32 page table."""
-    st = table.stride()
-    if table.dtype != torch.int32 or len(st) != 2 or (st[1] != 1 and table.shape[1] > 1):
-        raise B200KernelError(f"{what} must be int32 [sequences, columns] with unit column stride, got {table.dtype} "
-                              f"{tuple(table.shape)}")
-    rows, cols = table.shape
-    return rows, cols, st[0]
-
-
-def _output(out: torch.Tensor | None, like: torch.Tensor, what: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if out.shape != like.shape or out.dtype != like.dtype:
-        raise B200KernelError(f"{what} must have the input's shape {tuple(like.shape)} and dtype {like.dtype}")
-    return out
-
-
-def _rope_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, d: int) -> tuple[int, int, int]:
-    """(rows, leading dimension, rotary_dim) of the cos and sin tables."""
-    shape, st = cos.shape, cos.stride()
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(st) != 2 or shape != sin.shape
-            or st != sin.stride() or (st[1] != 1 and shape[1] > 1)):
-        raise B200KernelError(f"{what}: cos and sin must be fp32 [positions, rotary_dim / 2] of one layout")
-    rows, half = shape
-    if 2 * half > d:
-        raise B200KernelError(f"{what}: the tables rotate {2 * half} elements of heads of {d}")
-    return rows, st[0], 2 * half
+        so = load()
+        path = str(LIB_PATH.with_name("th_decode_ops.so"))
+        loader = machinery.ExtensionFileLoader("th_decode_ops", path)
+        try:
+            mod = util.module_from_spec(util.spec_from_file_location("th_decode_ops", path, loader=loader))
+            loader.exec_module(mod)
+        except ImportError as e:
+            raise B200KernelError(f"{path} does not load ({e}): rebuild with `python torch-helion_b200/build.py`") from None
+        mod.init(B200KernelError, *(ctypes.cast(getattr(so, f), _vp).value for f in (
+            "th_rope", "th_rope_append", "th_paged_attention", "th_paged_attention_workspace_size", "th_page_copy",
+            "th_last_error_string")))
+        _OPS = mod
+    return _OPS
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *,
@@ -482,30 +436,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: 
     turns back: the gradient with respect to the input is ``rope(grad, ..., inverse=True)``.  An output
     may be its input.  A negative position marks padding (zeros); one beyond the tables sets the device
     error word.  Returns ``(q_out, k_out)``."""
-    stream = _on_device("rope", q, k, positions, cos, sin, q_out, k_out)
-    q_tok, q_head = _heads(q, "rope: q")
-    tokens, hq, d = q.shape
-    rows, ld, rotary = _rope_tables("rope", cos, sin, d)
-    q_out = _output(q_out, q, "rope: q_out")
-    qo_tok, qo_head = _heads(q_out, "rope: q_out")
-    dtype = _dt(q)
-    k_args = (None, 0, 0, None, 0, 0)
-    hkv = 0
-    if k is not None:
-        k_tok, k_head = _heads(k, "rope: k")
-        k_tokens, hkv, dk = k.shape
-        if k.dtype != q.dtype or k_tokens != tokens or dk != d:
-            raise B200KernelError("rope: k must be [tokens, heads, head_dim] like q, of q's dtype")
-        k_out = _output(k_out, k, "rope: k_out")
-        k_args = (k.data_ptr(), k_tok, k_head, k_out.data_ptr(), *_heads(k_out, "rope: k_out"))
-    elif k_out is not None:
-        raise B200KernelError("rope: k_out without k")
-    at = _ints(positions, tokens, "rope: positions")
-    if tokens:
-        a = RopeArgs(q.data_ptr(), q_tok, q_head, q_out.data_ptr(), qo_tok, qo_head, *k_args, at, cos.data_ptr(),
-                     sin.data_ptr(), ld, tokens, rows, hq, hkv, d, rotary, bool(interleaved), bool(inverse), dtype)
-        _check(load().th_rope(ctypes.byref(a), stream), "th_rope")
-    return q_out, k_out
+    return (_OPS or _ops()).rope(q, k, positions, cos, sin, q_out, k_out, interleaved, inverse)
 
 
 def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
@@ -519,42 +450,8 @@ def rope_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positi
     pools [num_pages, hkv, page_size, d] (any page, head and slot strides).  A negative position marks
     padding: nothing is stored and its q_out row is zero.  Ids out of range set the device error word.
     ``k_out`` (optional, like k) receives the rotated keys as well.  Returns ``q_out`` (None without q)."""
-    stream = _on_device("rope_append", k, q, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out)
-    k_tok, k_head = _heads(k, "rope_append: k")
-    tokens, hkv, d = shape = k.shape
-    dt = k.dtype
-    if v.shape != shape or v.dtype != dt:
-        raise B200KernelError("rope_append: v must have k's shape and dtype")
-    rows, ld, rotary = _rope_tables("rope_append", cos, sin, d)
-    kp, vp, pool = _pool(k_pages, "rope_append: k_pages"), _pool(v_pages, "rope_append: v_pages"), k_pages.shape
-    if k_pages.dtype != dt or v_pages.dtype != dt or v_pages.shape != pool or pool[1] != hkv or pool[3] != d:
-        raise B200KernelError("rope_append: the pools must be [num_pages, hkv, page_size, d] of k's dtype")
-    q_args = (None, 0, 0, None, 0, 0)
-    hq = 0
-    if q is not None:
-        q_tok, q_head = _heads(q, "rope_append: q")
-        q_tokens, hq, dq = q.shape
-        if q.dtype != dt or q_tokens != tokens or dq != d:
-            raise B200KernelError("rope_append: q must be [tokens, heads, head_dim] like k, of k's dtype")
-        q_out = _output(q_out, q, "rope_append: q_out")
-        q_args = (q.data_ptr(), q_tok, q_head, q_out.data_ptr(), *_heads(q_out, "rope_append: q_out"))
-    elif q_out is not None:
-        raise B200KernelError("rope_append: q_out without q")
-    ko_args = (None, 0, 0)
-    if k_out is not None:
-        ko_args = (_output(k_out, k, "rope_append: k_out").data_ptr(), *_heads(k_out, "rope_append: k_out"))
-    batch, cols, ld_table = _page_table(table, "rope_append: table")
-    if seqs is None and batch < tokens:
-        raise B200KernelError(f"rope_append: {tokens} tokens without seqs need as many rows of table, got {batch}")
-    at = _ints(positions, tokens, "rope_append: positions")
-    of = None if seqs is None else _ints(seqs, tokens, "rope_append: seqs")
-    if tokens:
-        a = RopeArgs(*q_args, k.data_ptr(), k_tok, k_head, *ko_args, at, cos.data_ptr(), sin.data_ptr(), ld, tokens, rows,
-                     hq, hkv, d, rotary, bool(interleaved), 0, _dt(k), v.data_ptr(), *_heads(v, "rope_append: v"),
-                     k_pages.data_ptr(), *kp, v_pages.data_ptr(), *vp, table.data_ptr(), ld_table, of, batch, cols,
-                     pool[2], pool[0])
-        _check(load().th_rope_append(ctypes.byref(a), stream), "th_rope_append")
-    return q_out
+    return (_OPS or _ops()).rope_append(q, k, v, positions, cos, sin, k_pages, v_pages, table, seqs, q_out, k_out,
+                                        interleaved)
 
 
 def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor) -> torch.Tensor:
@@ -578,32 +475,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (fp32 [batch, hq], optional) receives log sum exp of the scores.  ``workspace`` comes from
     :func:`paged_attention_workspace` and may be kept; calls that share one must be ordered on the GPU
     (None: a fresh one per call)."""
-    stream = _on_device("paged_attention", q, k_pages, v_pages, table, lens, out, lse, workspace)
-    q_row, q_head = _heads(q, "paged_attention: q")
-    batch, hq, d = q.shape
-    dt = q.dtype
-    kp, vp, pool = _pool(k_pages, "paged_attention: k_pages"), _pool(v_pages, "paged_attention: v_pages"), k_pages.shape
-    num_pages, hkv, page_size, dk = pool
-    if v_pages.shape != pool or dk != d or k_pages.dtype != dt or v_pages.dtype != dt:
-        raise B200KernelError("paged_attention: the pools must be [num_pages, hkv, page_size, d] of q's dtype and head size")
-    rows, cols, ld = _page_table(table, "paged_attention: table")
-    if rows < batch:
-        raise B200KernelError(f"paged_attention: {batch} queries need as many rows of table, got {rows}")
-    out = _output(out, q, "paged_attention: out")
-    o_row, o_head = _heads(out, "paged_attention: out")
-    n = _ints(lens, batch, "paged_attention: lens")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (batch, hq) or not lse.is_contiguous()):
-        raise B200KernelError("paged_attention: lse must be contiguous fp32 [batch, hq]")
-    if batch == 0:
-        return out
-    if workspace is None:
-        workspace = paged_attention_workspace(q, k_pages)
-    a = PagedAttentionArgs(q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head, None if lse is None else lse.data_ptr(),
-                           k_pages.data_ptr(), *kp, v_pages.data_ptr(), *vp, table.data_ptr(), ld, n, batch, hq, hkv, d,
-                           page_size, num_pages, cols, window, d ** -0.5 if scale is None else scale, softcap, _dt(q),
-                           workspace.data_ptr(), workspace.nbytes)
-    _check(load().th_paged_attention(ctypes.byref(a), stream), "th_paged_attention")
-    return out
+    return (_OPS or _ops()).paged_attention(q, k_pages, v_pages, table, lens, out, scale, softcap, window, lse, workspace)
 
 
 def page_copy(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, counts: torch.Tensor | None = None) -> None:
@@ -613,16 +485,4 @@ def page_copy(pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, counts:
     plane that shares the page ids: layers x keys and values x heads), ``src``, ``dst`` and ``counts``
     int32 [pairs] (counts None: whole pages).  A negative id skips the pair.  Destinations must be
     distinct and none may be a source; ids out of range set the device error word."""
-    stream = _on_device("page_copy", pages, src, dst, counts)
-    shape, st = pages.shape, pages.stride()
-    if len(st) != 4 or st[3] != 1 or (st[2] != shape[3] and shape[2] > 1):
-        raise B200KernelError("page_copy: pages must be [num_pages, planes, page_size, width] with contiguous slots, got "
-                              f"shape {tuple(shape)} stride {st}")
-    if src.dim() != 1:
-        raise B200KernelError("page_copy: src must be one-dimensional")
-    n, es = src.shape[0], pages.element_size()
-    ids = _ints(src, n, "page_copy: src"), _ints(dst, n, "page_copy: dst"), None if counts is None else _ints(counts, n, "page_copy: counts")
-    if n == 0 or pages.numel() == 0:
-        return
-    a = PageCopyArgs(pages.data_ptr(), st[0] * es, st[1] * es, shape[3] * es, *ids, n, shape[0], shape[1], shape[2])
-    _check(load().th_page_copy(ctypes.byref(a), stream), "th_page_copy")
+    (_OPS or _ops()).page_copy(pages, src, dst, counts)
