@@ -43,19 +43,19 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
 // Transpose of an 8x8 matrix of 16-bit elements held in fragment order.
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ int atom_add_acq_rel(int* p, int v) {
@@ -123,7 +123,7 @@ struct PaScore {
 template <typename T_, int DP_, int NT, int KB_, int S_, int CTAS_>
 struct PaMma {
   using T = T_;
-  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16, FLY = NT == 1 ? 16 : 8;
+  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16, FLY = NT == 2 ? 8 : 16;
   static constexpr int SLOT = KB * DP * ES * 2, SHARED = 0;
   static constexpr int PASS = ROWS < KB ? ROWS : KB;  // rows of the accumulator that one block of the ring holds
   static_assert(PASS % 8 == 0, "whole mma columns");
@@ -181,46 +181,57 @@ struct PaMma {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
-    float s2[4] = {0.f, 0.f, 0.f, 0.f};  // a second chain where there is only one
+    // fragments of four k-steps at a time, so that loads and products overlap; where one mma a step is
+    // all there is, four partial sums instead of one long chain
+    constexpr int CHAINS = MT * NT == 1 ? 4 : MT * NT == 2 ? 2 : 1;
+    float part[CHAINS][MT * NT][4];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      if (kk * 16 >= d) break;
+    for (int h = 1; h < CHAINS; ++h)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        uint32_t a[4];
-        const int r = mt * 16 + (lane & 15);
-        ldsm_x4(ks + r * (DP * ES) + swz(r, kk * 2 + (lane >> 4)) * 16, a);
+      for (int f = 0; f < MT * NT; ++f)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (MT * NT == 1 && (kk & 1)) mma16816<T>(s2, a, q[kk][nt][0], q[kk][nt][1]);
-          else mma16816<T>(s[mt][nt], a, q[kk][nt][0], q[kk][nt][1]);
+        for (int e = 0; e < 4; ++e) part[h][f][e] = 0.f;
+#pragma unroll
+    for (int k4 = 0; k4 < DP / 16; k4 += 4) {
+      if (k4 * 16 >= d) break;
+      uint32_t a[4][MT][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const int r = mt * 16 + (lane & 15);
+          ldsm_x4(ks + r * (DP * ES) + swz(r, (k4 + j) * 2 + (lane >> 4)) * 16, a[j][mt]);
         }
-      }
-    }
-    if (MT * NT == 1) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][0][e] += s2[e];
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (j % CHAINS) mma16816<T>(part[j % CHAINS][mt * NT + nt], a[j][mt], q[k4 + j][nt][0], q[k4 + j][nt][1]);
+            else mma16816<T>(s[mt][nt], a[j][mt], q[k4 + j][nt][0], q[k4 + j][nt][1]);
+          }
     }
-    float mx[NT][2];
+    // The maximum that the exponentials are taken against is moved only when a score passes it by more
+    // than 8 (a factor of 256, far inside fp32's and the weights' range): most blocks need no exchange
+    // between the lanes and no rescaling.
     bool grew = false;
+    float mx[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      mx[nt][0] = m[nt][0];
-      mx[nt][1] = m[nt][1];
+      mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[mt][nt][e] = sc.template raw<ES>(s[mt][nt][e]);
+          float v = s[mt][nt][e];
+#pragma unroll
+          for (int h = 1; h < CHAINS; ++h) v += part[h][mt * NT + nt][e];
+          s[mt][nt][e] = v = sc.template raw<ES>(v);
           const bool live = (mask >> (mt * 16 + g + (e >> 1) * 8)) & 1;
-          mx[nt][e & 1] = fmaxf(mx[nt][e & 1], live ? s[mt][nt][e] * sc.mul : -INFINITY);
+          mx[nt][e & 1] = fmaxf(mx[nt][e & 1], live ? v * sc.mul : -INFINITY);
         }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int w = 4; w < 32; w *= 2) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], w));
-        grew |= mx[nt][e] > m[nt][e];
-      }
+      grew |= mx[nt][0] > m[nt][0] + 8.f || mx[nt][1] > m[nt][1] + 8.f;
     }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -228,9 +239,12 @@ struct PaMma {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          f[e] = m[nt][e] == -INFINITY ? 0.f : ex2_fast(m[nt][e] - mx[nt][e]);
+          float top = fmaxf(mx[nt][e], m[nt][e]);
+#pragma unroll
+          for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          f[e] = m[nt][e] == -INFINITY ? 0.f : ex2_fast(m[nt][e] - top);
           l[nt][e] *= f[e];
-          m[nt][e] = mx[nt][e];
+          m[nt][e] = top;
         }
 #pragma unroll
         for (int dt = 0; dt < DP / 16; ++dt)
@@ -256,20 +270,22 @@ struct PaMma {
         }
     }
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; ++dt) {
-      if (dt * 16 >= d) break;
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        uint32_t a[4];
+      for (int d4 = 0; d4 < DP / 16; d4 += 4) {
+        if (d4 * 16 >= d) break;
+        uint32_t a[4][4];
         const int r = mt * 16 + (lane & 7) + ((lane >> 4) << 3);
-        ldsm_x4_trans(vs + r * (DP * ES) + swz(r, dt * 2 + ((lane >> 3) & 1)) * 16, a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ldsm_x4_trans(vs + r * (DP * ES) + swz(r, (d4 + j) * 2 + ((lane >> 3) & 1)) * 16, a[j]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma16816<T>(o[dt][nt], a, hi[mt][nt][0], hi[mt][nt][1]);
-          mma16816<T>(o[dt][nt], a, lo[mt][nt][0], lo[mt][nt][1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16816<T>(o[d4 + j][nt], a[j], hi[mt][nt][0], hi[mt][nt][1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16816<T>(o[d4 + j][nt], a[j], lo[mt][nt][0], lo[mt][nt][1]);
         }
       }
-    }
   }
 
   __device__ __forceinline__ void stats(float2* ml) {
@@ -356,28 +372,32 @@ struct PaSimt {
       }
     }
     const bool live = (mask >> r) & 1;
-    float f[NH];
     bool grew = false;
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       s[h] += __shfl_xor_sync(0xffffffffu, s[h], 1);
       s[h] += __shfl_xor_sync(0xffffffffu, s[h], 2);
       s[h] = sc.template raw<ES>(s[h]);
-      float mx = fmaxf(m[h], live ? s[h] * sc.mul : -INFINITY);
-#pragma unroll
-      for (int w = 4; w < 32; w *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-      f[h] = m[h] == -INFINITY ? 0.f : ex2_fast(m[h] - mx);
-      grew |= mx > m[h];
-      m[h] = mx;
-      const float p = live ? ex2_fast(fmaf(s[h], sc.mul, mx == -INFINITY ? 0.f : -mx)) : 0.f;
-      l[h] = fmaf(l[h], f[h], p);
-      if (c == 0) ps[r * NH + h] = p;
+      grew |= live && s[h] * sc.mul > m[h] + 8.f;  // as in PaMma::tile
     }
-    if (grew) {  // the maxima are the same in every lane
+    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h)
+      for (int h = 0; h < NH; ++h) {
+        float top = fmaxf(m[h], live ? s[h] * sc.mul : -INFINITY);
 #pragma unroll
-        for (int e = 0; e < EL; ++e) o[h][e] *= f[h];
+        for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        const float f = m[h] == -INFINITY ? 0.f : ex2_fast(m[h] - top);
+        m[h] = top;
+        l[h] *= f;
+#pragma unroll
+        for (int e = 0; e < EL; ++e) o[h][e] *= f;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      const float p = live ? ex2_fast(fmaf(s[h], sc.mul, m[h] == -INFINITY ? 0.f : -m[h])) : 0.f;
+      l[h] += p;
+      if (c == 0) ps[r * NH + h] = p;
     }
     __syncwarp();
 #pragma unroll
@@ -759,7 +779,7 @@ static auto pa_dispatch(int dtype, int head_dim, int group, F&& f) {
     }
     if (head_dim <= 128) {
       if (group <= 8) return f(PaKind<PaMma<T, 128, 1, 16, 2, 3>>{});
-      if (group <= 16) return f(PaKind<PaMma<T, 128, 2, 16, 2, 3>>{});
+      if (group <= 16) return f(PaKind<PaMma<T, 128, 2, 16, 3, 2>>{});
       if (group <= 24) return f(PaKind<PaMma<T, 128, 3, 16, 3, 2>>{});
       return f(PaKind<PaMma<T, 128, 4, 16, 3, 2>>{});
     }
