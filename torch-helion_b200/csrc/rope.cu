@@ -118,7 +118,7 @@ union RopeChunk {
 // head past rotary_dim pass through.  A block takes TOK tokens; the cache
 // slots of its tokens are looked up once, behind the first rows' loads, and
 // each row's loads are issued before the row before it is stored.
-constexpr int ROPE_TOK = 4;
+constexpr int ROPE_TOK = 8;
 
 template <typename T, bool APPEND, bool INTER>
 __global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ th_rope_args p, int tok, int shift) {
@@ -294,7 +294,7 @@ static int rope_launch(const th_rope_args* a, cudaStream_t st, const char* what)
     const int busy = (a->head_dim / (16 / (int)sizeof(T)) + 1) / 2;  // lanes that a row keeps busy
     int shift = 0;
     while (shift < 5 && (1 << shift) < busy) ++shift;
-    const int tok = a->tokens >= 4 * 2 * (int64_t)sm_count() ? ROPE_TOK : 1;
+    const int tok = a->tokens >= ROPE_TOK * 2 * (int64_t)sm_count() ? ROPE_TOK : 1;
     const int64_t blocks = (a->tokens + tok - 1) / tok;
     if (blocks > INT32_MAX) return fail(TH_EUNSUPPORTED, "%s: too many tokens", what);
     auto k = a->interleaved ? rope_vec_kernel<T, APPEND, true> : rope_vec_kernel<T, APPEND, false>;
