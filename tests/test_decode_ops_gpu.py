@@ -128,6 +128,31 @@ def test_rope_gradient(L, interleaved):
         assert abs(slope - float((got.double() * e.double()).sum())) < 1e-4
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_function_gives_gradients(L, interleaved):
+    """Rotary.apply against autograd of the 64-bit form: both outputs used, one of them only, none of k, and a
+    gradient that arrives broadcast (the sum's)."""
+    from torch_helion.b200.kv_cache import Rotary
+
+    cos, sin = tables(L, 64, 48)
+    pos = ints([3, 0, 63, -1, 8])
+    gq, gk = rand(5, 6, 64, seed=1).double(), rand(5, 2, 64, seed=2).double()
+    for use_q, use_k, have_k in ((True, True, True), (True, False, True), (False, True, True), (True, False, False)):
+        q, k = rand(5, 6, 64, seed=3).requires_grad_(), rand(5, 2, 64, seed=4).requires_grad_()
+        q64, k64 = q.detach().double().requires_grad_(), k.detach().double().requires_grad_()
+        qo, ko = Rotary.apply(q, k if have_k else None, pos, cos, sin, interleaved)
+        assert (ko is None) == (not have_k)
+        ref = (rope64(q64, pos, cos, sin, interleaved) * gq).sum() * use_q
+        got = (qo * gq.float()).sum() * use_q
+        if use_k:
+            ref, got = ref + rope64(k64, pos, cos, sin, interleaved).sum(), got + ko.sum()
+        ref.backward()
+        got.backward()
+        for x, y in ((q, q64), (k, k64)):
+            if y.grad is not None:
+                assert rel_l2(x.grad, y.grad) <= 2**-22 if float(y.grad.norm()) else float(x.grad.norm()) == 0
+
+
 def test_rope_position_beyond_the_tables(L):
     q = rand(4, 2, 64, dtype=torch.bfloat16)
     cos, sin = tables(L, 16, 64)
@@ -338,6 +363,33 @@ def test_attention_infinite_and_nan_values(L, dtype):
     got = L.paged_attention(rand(3, 4, 64, dtype=dtype), kp, vp, table, n)
     assert bool(got[0, :2].isnan().all()) and bool(got[1, 2:].isnan().all())
     assert torch.equal(got[0, 2:], clean[0, 2:]) and torch.equal(got[1, :2], clean[1, :2]) and torch.equal(got[2], clean[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_nan_key_under_a_cap(L, dtype):
+    """A cap does not turn a NaN score into a number; an infinite score becomes the cap."""
+    kp, vp, table, n = cached([100, 40], 1, 64, 16, dtype)
+    q = rand(2, 4, 64, dtype=dtype)
+    kp[table[0, 2], 0, 5, 7] = float("nan")
+    got = L.paged_attention(q, kp, vp, table, n, softcap=20.0)
+    assert bool(got[0].isnan().all()) and not bool(got[1].isnan().any())
+    kp[table[0, 2], 0, 5] = 0.0
+    kp[table[0, 2], 0, 5, 7] = float("inf")
+    q[:, :, 7] = 1.0
+    check_attend(L, q, kp, vp, table, n, softcap=20.0)
+
+
+def test_attention_one_workspace_for_several_kinds(L):
+    """Calls of other head sizes, groups and types may use one workspace in turn, if it is large enough for each."""
+    cases = []
+    for hq, hkv, d, dtype in ((8, 2, 128, torch.bfloat16), (40, 1, 128, torch.float16), (4, 4, 64, torch.float32), (6, 1, 256, torch.bfloat16)):
+        kp, vp, table, n = cached([7000, 1, 900], hkv, d, 16, dtype)
+        q = rand(3, hq, d, dtype=dtype)
+        cases.append((q, kp, vp, table, n, L.paged_attention(q, kp, vp, table, n)))
+    ws = max((L.paged_attention_workspace(c[0], c[1]) for c in cases), key=lambda w: w.numel())
+    for _ in range(3):
+        for q, kp, vp, table, n, want in cases:
+            assert torch.equal(L.paged_attention(q, kp, vp, table, n, workspace=ws), want)
 
 
 def test_attention_lengths_and_pages_out_of_range(L):

@@ -73,6 +73,33 @@ def rope_tables(positions: int, rotary_dim: int, theta: float = 10000.0, *, scal
     return (angle.cos() * gain).float(), (angle.sin() * gain).float()
 
 
+class Rotary(torch.autograd.Function):
+    """:func:`lib.rope` with its gradient: ``q, k = Rotary.apply(q, k, positions, cos, sin, interleaved)``.
+
+    The rotation is linear and orthogonal up to the tables' factor, so the gradient with respect to an
+    input is the opposite rotation of the gradient with respect to its output; nothing but the tables
+    and positions is kept.  k may be None."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, cos, sin, interleaved=False):
+        ctx.save_for_backward(positions, cos, sin)
+        ctx.interleaved = interleaved
+        return lib.rope(q, k, positions, cos, sin, interleaved=interleaved)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, cos, sin = ctx.saved_tensors
+        kw = {"interleaved": ctx.interleaved, "inverse": True}
+        # a missing output's gradient is None; broadcast ones (stride 0) are laid out first
+        dq = None if dq is None else dq.contiguous()
+        dk = None if dk is None else dk.contiguous()
+        if dq is None and dk is not None:
+            dk, _ = lib.rope(dk, None, positions, cos, sin, **kw)
+        elif dq is not None:
+            dq, dk = lib.rope(dq, dk, positions, cos, sin, **kw)
+        return dq, dk, None, None, None, None
+
+
 @dataclass
 class Step:
     """Device inputs of one step over a batch of sequences (all int32)."""

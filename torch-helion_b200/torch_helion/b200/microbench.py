@@ -6,12 +6,21 @@
     python -m torch_helion.b200.microbench gemm --m 8192 --n 3328 --k 768 --vs-torch
     python -m torch_helion.b200.microbench conv --batch 4 --seq 2048 --channels 1792
     python -m torch_helion.b200.microbench rmsnorm --m 8192 --k 768
+    python -m torch_helion.b200.microbench decode --batch 64 --seq 4096 --hq 32 --hkv 8 --head-dim 128 --page 16
+    python -m torch_helion.b200.microbench rope --batch 8 --seq 4096
+    python -m torch_helion.b200.microbench append --batch 8 --seq 2048
+    python -m torch_helion.b200.microbench page-copy --m 512 --n 512
     torchrun --nproc-per-node 8 -m torch_helion.b200.microbench allreduce --rows 32768 --cols 4096 --ctas 16,24,32
 
 Each mode runs 3 warm-up launches and times ``--iters`` launches with CUDA
 events (L2 flushed before each when ``--flush``), printing one JSON line with
 the median time and the kernel's algorithmic throughput.  This is the
 command behind the single-kernel ncu captures.
+
+``decode`` is attention of one new token for each of ``--batch`` sequences of
+``--seq`` cached tokens, ``rope`` and ``append`` rotate (and store in pages)
+``--batch`` x ``--seq`` tokens of ``--hq`` + ``--hkv`` heads, ``page-copy`` copies
+``--m`` pages of ``--n`` planes of ``--page`` slots of 128 bf16.
 
 ``allreduce`` (one process per GPU under torchrun) sums a bf16 [rows, cols] array
 over the ranks with ``th_allreduce`` for every ``--ctas`` grid size and
@@ -104,6 +113,40 @@ def _ssd_sweep(a) -> None:
             torch.cuda.empty_cache()
 
 
+def _decode_case(a):
+    """(launch, algorithmic bytes) of the cached-decoding operators on seeded bf16 operands, pages in random order."""
+    from .kv_cache import rope_tables
+
+    dev, bf = "cuda", torch.bfloat16
+    row = a.head_dim * 2
+    if a.kernel == "page-copy":
+        pages = torch.randn(2 * a.m, a.n, a.page, 128, device=dev, dtype=bf)
+        order = torch.randperm(2 * a.m, device=dev).int()
+        src, dst = order[: a.m].clone(), order[a.m :].clone()
+        return lambda: lib.page_copy(pages, src, dst), 2.0 * a.m * a.n * a.page * 256
+    tokens = a.batch * a.seq
+    cols = -(-a.seq // a.page)
+    if a.kernel != "rope":
+        kv = torch.randn(2, a.batch * cols, a.hkv, a.page, a.head_dim, device=dev, dtype=bf)
+        table = torch.randperm(a.batch * cols, device=dev).int().view(a.batch, cols)
+    if a.kernel == "decode":
+        q = torch.randn(a.batch, a.hq, a.head_dim, device=dev).to(bf)
+        lens = torch.full((a.batch,), a.seq, dtype=torch.int32, device=dev)
+        ws, o = lib.paged_attention_workspace(q, kv[0]), torch.empty_like(q)
+        return (lambda: lib.paged_attention(q, kv[0], kv[1], table, lens, o, workspace=ws),
+                2.0 * tokens * a.hkv * row + 2.0 * a.batch * a.hq * row)
+    qkv = torch.randn(tokens, a.hq + 2 * a.hkv, a.head_dim, device=dev, dtype=bf)
+    q, k, v = qkv[:, : a.hq], qkv[:, a.hq : a.hq + a.hkv], qkv[:, a.hq + a.hkv :]
+    pos = torch.arange(a.seq, device=dev, dtype=torch.int32).repeat(a.batch)
+    cos, sin = rope_tables(a.seq, a.head_dim, device=dev)
+    q_out, k_out = torch.empty(q.shape, device=dev, dtype=bf), torch.empty(k.shape, device=dev, dtype=bf)
+    if a.kernel == "rope":
+        return lambda: lib.rope(q, k, pos, cos, sin, q_out=q_out, k_out=k_out), 2.0 * tokens * (a.hq + a.hkv) * row
+    seqs = torch.arange(a.batch, device=dev, dtype=torch.int32).repeat_interleave(a.seq)
+    return (lambda: lib.rope_append(q, k, v, pos, cos, sin, kv[0], kv[1], table, seqs=seqs, q_out=q_out),
+            2.0 * tokens * (a.hq + 2 * a.hkv) * row)
+
+
 def _allreduce(a) -> None:
     import os
     from datetime import timedelta
@@ -157,7 +200,7 @@ def _allreduce(a) -> None:
 def main(argv=None) -> None:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("kernel", choices=["attention", "ssd", "ssd-sweep", "gemm", "conv", "rmsnorm", "rowstat",
-                                       "allreduce"])
+                                       "allreduce", "decode", "rope", "append", "page-copy"])
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seq", type=int, default=4096)
     ap.add_argument("--hq", type=int, default=32)
@@ -171,6 +214,7 @@ def main(argv=None) -> None:
     ap.add_argument("--k", type=int, default=768)
     ap.add_argument("--channels", type=int, default=1792)
     ap.add_argument("--iters", type=int, default=20)
+    ap.add_argument("--page", type=int, default=16, help="decode, append, page-copy: slots of a page")
     ap.add_argument("--ctas", default="16,24,32", help="allreduce: th_allreduce grid sizes to time")
     # (not --m / --k: under torchrun those would be taken for abbreviations of its own options)
     ap.add_argument("--rows", type=int, default=32768, help="allreduce: rows of the bf16 array")
@@ -191,7 +235,10 @@ def main(argv=None) -> None:
     if a.kernel == "allreduce":
         _allreduce(a)
         return
-    if a.kernel == "attention":
+    if a.kernel in ("decode", "rope", "append", "page-copy"):
+        fn, work = _decode_case(a)
+        unit = "GB/s"
+    elif a.kernel == "attention":
         t = a.batch * a.seq
         q = torch.randn(t, a.hq * a.head_dim, device=dev).to(bf)
         k = torch.randn(t, a.hkv * a.head_dim, device=dev).to(bf)
