@@ -2,7 +2,7 @@
 // append of rotated keys and of values to a paged cache.
 #include <type_traits>
 
-#include "/root/repo/torch-helion_b200/csrc/common.cuh"
+#include "common.cuh"
 
 namespace th {
 
