@@ -22,12 +22,13 @@
 //
 // Measured on a B200 (32 heads over 8, head 128, bf16): four sequences of about
 // 100k tokens 300 us, 6.7 TB/s of keys and values, the rate of a plain copy; 64
-// ragged sequences (17 to 8191 tokens) 81 us, 4.8 TB/s: every run ends in the
-// middle of an item, about 4 us, and 16 of the 148 SMs reach memory 12 % slower
+// ragged sequences (17 to 8191 tokens) 74 us, 5.2 TB/s: every run ends in the
+// middle of an item, a few us, and 16 of the 148 SMs reach memory 12 % slower
 // than the rest, which equal runs wait for.  Handing out the last eighth of the
 // runs to whichever CTA is free was tried and costs in ends what it gains.  One
 // sequence of 4097 tokens takes 14 us: the chain length, page, key, product,
-// part, join, of about a microsecond each.
+// part, join, of about a microsecond each; 4000 sequences of 40 tokens 283 us
+// (655 MB), nearly all of it the ends of items.
 #include "common.cuh"
 
 namespace th {
@@ -526,17 +527,39 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
   const int group = p.hq / p.hkv, items = p.hkv * x.chunks, d = p.head_dim, dch = d * P::ES / 16;
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0)
+    for (int i = tid; i < p.batch; i += PA_WARPS * 32)
+      if (p.lens[i] > x.capacity) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
+
+  // Tiles of 32 sequences each, in lane k those of the k-th 32 of 1024 from g0
+  // (32 sequences of 2^26 tiles fit); the lengths are asked for side by side.
+  auto sums = [&](int g0) {
+    unsigned mine = 0;
+    const int blocks = min(32, (p.batch - g0 + 31) / 32);
+#pragma unroll 8
+    for (int k = 0; k < blocks; ++k) {
+      const int i = g0 + k * 32 + lane;
+      const unsigned n = i < p.batch ? pa_tiles(pa_kept(pa_clean(p.lens[i], x), p.window), TILE) : 0;
+      const unsigned sum = __reduce_add_sync(0xffffffffu, n);
+      if (lane == k) mine = sum;
+    }
+    return mine;
+  };
+  auto scan = [&](auto v) {  // inclusive, over the lanes
+#pragma unroll
+    for (int s = 1; s < 32; s *= 2) {
+      const auto y = __shfl_up_sync(0xffffffffu, v, s);
+      if (lane >= s) v += y;
+    }
+    return v;
+  };
 
   // this CTA's run of tiles [u0, u0 + n)
   long long total = 0;
-  for (int base = 0; base < p.batch; base += 32) {
-    unsigned n = 0;  // 32 sequences of 2^26 tiles fit
-    if (base + lane < p.batch) {
-      const int len = p.lens[base + lane];
-      if (len > x.capacity && blockIdx.x == 0 && warp == 0) atomicOr(&g_device_error, TH_DEVERR_BAD_ARG);
-      n = pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE);
-    }
-    total += __reduce_add_sync(0xffffffffu, n);
+  unsigned mine = 0;
+  for (int g0 = 0; g0 < p.batch; g0 += 1024) {
+    mine = sums(g0);
+    total += p.batch <= 32 ? (long long)__shfl_sync(0xffffffffu, mine, 0) : __shfl_sync(0xffffffffu, scan((long long)mine), 31);
   }
   const long long W = total * items;
   // as few CTAs as still finish in the same number of tiles: one sequence of 4097 tokens and 8 key-value
@@ -549,26 +572,28 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
   const int n = (int)(split.first(c + 1) - u0);
   PaWalk w;
   {
-    long long before = 0;
-    for (int base = 0;; base += 32) {
-      const int len = base + lane < p.batch ? p.lens[base + lane] : 0;
-      const unsigned nt = base + lane < p.batch ? pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE) : 0;
-      unsigned incl = nt;
-#pragma unroll
-      for (int s = 1; s < 32; s *= 2) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, incl, s);
-        if (lane >= s) incl += y;
+    long long before = 0;  // tiles of the sequences before the 32 from b0
+    int b0 = 0;
+    if (p.batch > 32) {
+      for (int g0 = 0;; g0 += 1024) {
+        if (p.batch > 1024) mine = sums(g0);
+        const long long to = scan((long long)mine);
+        const unsigned hit = __ballot_sync(0xffffffffu, (before + to) * items > u0);
+        if (hit) {
+          const int k = __ffs(hit) - 1;
+          b0 = g0 + k * 32;
+          before += __shfl_sync(0xffffffffu, to - mine, k);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, to, 31);
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, (before + incl) * items > u0);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        w.b = base + src;
-        before += __shfl_sync(0xffffffffu, incl - nt, src);
-        pa_enter(w, p, x, __shfl_sync(0xffffffffu, len, src), TILE);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
     }
+    const int len = b0 + lane < p.batch ? p.lens[b0 + lane] : 0;
+    const unsigned nt = b0 + lane < p.batch ? pa_tiles(pa_kept(pa_clean(len, x), p.window), TILE) : 0, incl = scan(nt);
+    const int src = __ffs(__ballot_sync(0xffffffffu, (before + incl) * items > u0)) - 1;
+    w.b = b0 + src;
+    before += __shfl_sync(0xffffffffu, incl - nt, src);
+    pa_enter(w, p, x, __shfl_sync(0xffffffffu, len, src), TILE);
     const long long in = u0 - before * items;
     w.hc = (int)PaSplit::div(in, w.nt);
     w.t = (int)(in - (long long)w.hc * w.nt);
@@ -693,6 +718,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
         pa_store4(o, v, ll == 0.f ? 0.f : 1.f / ll, x.o_quads);
         if (p.lse && dd == 0) p.lse[(int64_t)b * p.hq + h0 + r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
       };
+      // the next item's queries arrive while this one is finished; shared ones once all warps are past them
+      const int4 next = sm_meta[warp][at + 1 == S ? 0 : at + 1];
+      if (!P::SHARED && i + 1 < n) load_q(next.x, next.y);
       acc.stats(sm_ml[warp]);
       __syncwarp();
 #pragma unroll
@@ -724,10 +752,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
           }
         }
       }
-      if (i + 1 < n) {  // the next item's queries arrive while this one is finished
-        const int4 next = sm_meta[warp][at + 1 == S ? 0 : at + 1];
-        load_q(next.x, next.y);
-      }
+      if (P::SHARED && i + 1 < n) load_q(next.x, next.y);
       if (!whole) {
         // the CTAs on this item: those whose runs meet its tiles
         const long long ub = u0 + i - meta.z;
@@ -796,7 +821,7 @@ struct PaKind { using type = P; };
 // a kind holds as many query heads of a group as its registers allow.  Three
 // CTAs an SM with rings of two blocks beat two with rings of three wherever the
 // accumulators leave room (64 ragged sequences of 32 heads over 8, head 128: 81
-// against 97 us; four of 100k tokens: 300 against 337): twelve warps hide one
+// against 97 us when it was tried; four of 100k tokens: 300 against 337): twelve warps hide one
 // another's products better than a third block hides the copies.
 template <typename F>
 static auto pa_dispatch(int dtype, int head_dim, int group, F&& f) {
@@ -863,7 +888,9 @@ static int pa_launch(const th_paged_attention_args* a, PaPlan x, cudaStream_t st
   x.chunks = (a->hq / a->hkv + P::ROWS - 1) / P::ROWS;
   const size_t smem = (size_t)PA_WARPS * P::S * P::SLOT + P::SHARED;
   if (int rc = smem_limit(paged_attention_kernel<P>, smem, "th_paged_attention")) return rc;
-  launch_pdl(paged_attention_kernel<P>, dim3(sm_count() * P::CTAS), dim3(PA_WARPS * 32), smem, st, *a, x);
+  // no more CTAs than tiles that the table has room for
+  const int64_t tiles = (int64_t)a->batch * a->hkv * x.chunks * ((x.capacity - 1) / (PA_WARPS * P::KB) + 1), most = (int64_t)sm_count() * P::CTAS;
+  launch_pdl(paged_attention_kernel<P>, dim3((unsigned)(tiles < most ? tiles : most)), dim3(PA_WARPS * 32), smem, st, *a, x);
   return check_launch("th_paged_attention");
 }
 
