@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import heapq
 import math
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -124,7 +125,7 @@ class PagedKVCache:
         self.data = torch.empty(num_pages, layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=self.device)
         self._refs = [0] * num_pages
         self._free = list(range(num_pages))  # a heap: the lowest free id first keeps the pool's front dense
-        self._pages: dict[int, list[int]] = {}
+        self._pages: dict[int, array] = {}  # of C ints, as the table's rows are
         self._len: dict[int, int] = {}
         self._next = 0
         self._workspace: dict[int, torch.Tensor] = {}
@@ -145,7 +146,7 @@ class PagedKVCache:
         """An empty sequence."""
         seq = self._next
         self._next += 1
-        self._pages[seq], self._len[seq] = [], 0
+        self._pages[seq], self._len[seq] = array("i"), 0
         return seq
 
     def _take(self) -> int:
@@ -169,26 +170,26 @@ class PagedKVCache:
         more = sum(n - len(self._pages[s]) for s, n in zip(seqs, need))
         if more > len(self._free):
             raise CacheFull(f"{more} pages are needed, {len(self._free)} are free")
-        positions: list[int] = []
-        rows: list[int] = []
-        for r, (s, n, k) in enumerate(zip(seqs, need, counts)):
-            self._pages[s] += [self._take() for _ in range(n - len(self._pages[s]))]
-            positions += range(self._len[s], self._len[s] + k)
-            rows += [r] * k
-            self._len[s] += k
+        before = torch.tensor([self._len[s] for s in seqs], dtype=torch.int32)
+        new = torch.tensor(counts, dtype=torch.int32)
         cols = max(1, max(need))
         table = torch.full((len(seqs), cols), -1, dtype=torch.int32)
-        for r, s in enumerate(seqs):
-            table[r, : len(self._pages[s])] = torch.tensor(self._pages[s], dtype=torch.int32)
-        lens = torch.tensor([self._len[s] for s in seqs], dtype=torch.int32)
+        for r, (s, n, k) in enumerate(zip(seqs, need, counts)):
+            pages = self._pages[s]
+            pages.extend(self._take() for _ in range(n - len(pages)))
+            self._len[s] += k
+            if n:
+                table[r, :n] = torch.frombuffer(pages, dtype=torch.int32)
+        rows = torch.repeat_interleave(torch.arange(len(seqs), dtype=torch.int32), new)
+        first = torch.cumsum(new, 0, dtype=torch.int32) - new  # of each sequence's tokens
+        positions = torch.arange(rows.shape[0], dtype=torch.int32) + (before - first)[rows]
         # one buffer, one copy; torch's pinned allocator keeps the staging memory until the copy has run
-        host = torch.cat((torch.tensor(positions, dtype=torch.int32), torch.tensor(rows, dtype=torch.int32), lens,
-                          table.reshape(-1)))
+        host = torch.cat((positions, rows, before + new, table.reshape(-1)))
         if self.device.type == "cuda":
             dev = host.pin_memory().to(self.device, non_blocking=True)
         else:
             dev = host
-        a, b = len(positions), len(seqs)
+        a, b = rows.shape[0], len(seqs)
         return Step(dev[:a], dev[a : 2 * a], dev[2 * a : 2 * a + b], dev[2 * a + b :].view(b, cols))
 
     def fork(self, seq: int, n: int = 1) -> list[int]:
@@ -241,7 +242,7 @@ class PagedKVCache:
         for src, dst in moved.items():
             self._refs[dst], self._refs[src] = self._refs[src], 0
         for s, pages in self._pages.items():
-            self._pages[s] = [moved.get(p, p) for p in pages]
+            self._pages[s] = array("i", (moved.get(p, p) for p in pages))
         self._free = list(range(live, self.num_pages))
         return len(moved)
 
