@@ -366,7 +366,8 @@ int th_rope_append(const th_rope_args* a, void* stream);
  * 16 bytes (head_dim <= 256), the pools 16-byte aligned in base and strides.
  * The workspace (th_paged_attention_workspace_size bytes, 16-byte aligned)
  * must be zero before its first use; every call leaves its counters at zero,
- * so it can be kept.  Calls that share one must not overlap on the GPU. */
+ * so it can be kept, also for calls with other heads and types if it is large
+ * enough for them.  Calls that share one must not overlap on the GPU. */
 typedef struct {
   const void* q;        int64_t q_row, q_head;
   void* o;              int64_t o_row, o_head;

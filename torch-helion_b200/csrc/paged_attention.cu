@@ -22,12 +22,12 @@
 //
 // Measured on a B200 (32 heads over 8, head 128, bf16): four sequences of about
 // 100k tokens 300 us, 6.7 TB/s of keys and values, the rate of a plain copy; 64
-// ragged sequences (17 to 8191 tokens) 74 us, 5.2 TB/s: every run ends in the
+// ragged sequences (17 to 8191 tokens) 72 us, 5.4 TB/s: every run ends in the
 // middle of an item, a few us, and 16 of the 148 SMs reach memory 12 % slower
 // than the rest, which equal runs wait for.  Handing out the last eighth of the
 // runs to whichever CTA is free was tried and costs in ends what it gains.  One
 // sequence of 4097 tokens takes 14 us: the chain length, page, key, product,
-// part, join, of about a microsecond each; 4000 sequences of 40 tokens 283 us
+// part, join, of about a microsecond each; 4000 sequences of 40 tokens 268 us
 // (655 MB), nearly all of it the ends of items.
 #include "common.cuh"
 
@@ -95,7 +95,6 @@ struct PaPlan {
   int capacity;   // keys a table row can name
   int chunks;     // blocks of query heads per key-value head
   int page_shift; // log2 of the page size, or -1
-  int same;       // both pools have the same strides
   int q_pairs;    // q may be read two elements at a time
   int o_quads;    // o may be written four elements at a time
   float* partial; // [2 CTAs][rows][DP]: of CTA c the item it ends inside (2 c + 1) or came into (2 c)
@@ -140,7 +139,8 @@ struct PaScore {
 template <typename T_, int DP_, int NT, int KB_, int S_, int CTAS_>
 struct PaMma {
   using T = T_;
-  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16, FLY = NT == 2 ? 8 : 16;
+  static constexpr int DP = DP_, KB = KB_, S = S_, CTAS = CTAS_, ROWS = 8 * NT, ES = 2, MT = KB / 16;
+  static constexpr int FLY = NT <= 2 ? 8 : 16;  // parts in flight in a join: more registers there slow the whole loop of the small kinds
   static constexpr int SLOT = KB * DP * ES * 2, SHARED = 0;
   static constexpr int PASS = ROWS < KB ? ROWS : KB;  // rows of the accumulator that one block of the ring holds
   static_assert(PASS % 8 == 0, "whole mma columns");
@@ -631,13 +631,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, P::CTAS)
     const bool all = mask == 0xffffffffu >> (32 - KB) && dch == CH;
     const int hk = x.chunks == 1 ? k.hc : k.hc / x.chunks;
     const long long ko = live ? page * p.k_page + slot * p.k_slot + hk * p.k_head : 0;
-    const long long vo = live && !x.same ? page * p.v_page + slot * p.v_slot + hk * p.v_head : 0;
+    const long long vo = live ? page * p.v_page + slot * p.v_slot + hk * p.v_head : 0;
     const uint32_t dst = ring_u + at * P::SLOT + (lane >> 3) * (DP * P::ES);
 #pragma unroll
     for (int i = 0; i < KB / 4; ++i) {
       const int row = i * 4 + (lane >> 3);
       const long long ki = __shfl_sync(0xffffffffu, ko, row);
-      const long long vi = x.same ? ki : __shfl_sync(0xffffffffu, vo, row);
+      const long long vi = __shfl_sync(0xffffffffu, vo, row);
       const bool ok = (mask >> row) & 1;
       const T* ka = kp + ki + sub * (16 / P::ES);
       const T* va = vp + vi + sub * (16 / P::ES);
@@ -924,7 +924,6 @@ extern "C" int th_paged_attention(const th_paged_attention_args* a, void* stream
   const int64_t cap = (int64_t)a->table_cols * a->page_size;
   x.capacity = (int)(cap < INT32_MAX - 4096 ? cap : INT32_MAX - 4096);
   x.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctz(a->page_size) : -1;
-  x.same = a->k_page == a->v_page && a->k_head == a->v_head && a->k_slot == a->v_slot;
   x.q_pairs = reinterpret_cast<uintptr_t>(a->q) % 4 == 0 && a->q_row % 2 == 0 && a->q_head % 2 == 0;
   x.o_quads = reinterpret_cast<uintptr_t>(a->o) % (4 * eb) == 0 && a->o_row % 4 == 0 && a->o_head % 4 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
