@@ -77,7 +77,7 @@ def _binding_command(out: Path) -> list[str]:
     include = [root / "include", root / "include/torch/csrc/api/include", cuda / "include", sysconfig.get_paths()["include"]]
     return [os.environ.get("CXX", "g++"), *CXX_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             *(x for d in include for x in ("-isystem", str(d))), str(CSRC / "decode_ops.cpp"), "-o", str(out),
-            "-L" + str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+            "-L" + str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

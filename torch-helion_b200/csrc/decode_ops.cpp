@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -128,7 +129,7 @@ const int32_t* page_table(const Tensor& t, const char* op, int32_t& rows, int32_
 // `out`, or a new contiguous tensor like `like` held in `made`.
 const Tensor& output(const Tensor* out, const Tensor& like, Name n, std::optional<Tensor>& made) {
   if (!out) {
-    made = at::empty_like(like, at::TensorOptions(), at::MemoryFormat::Contiguous);
+    made = at::detail::empty_cuda(like.sizes(), like.scalar_type(), like.device(), std::nullopt);  // contiguous
     return *made;
   }
   if (out->sizes() != like.sizes() || out->scalar_type() != like.scalar_type())
