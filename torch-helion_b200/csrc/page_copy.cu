@@ -1,5 +1,8 @@
 // th_page_copy: copies of pages, or of their first slots, inside one pool.
-// Bound by memory: every byte is read once and written once.
+// Bound by memory: every byte is read once and written once.  On a B200 509
+// pages of 2 MB take 317 us, 6.7 TB/s of reads and writes, the rate of a plain
+// copy; 64 partly filled ones of 512 planes 20 us on the device, 6.0 TB/s.  One
+// block per plane with a load and a store at a time took 345 and 33 us.
 #include "common.cuh"
 
 namespace th {

@@ -8,8 +8,8 @@
 // below it.  The kernel is a stream of cp.async copies with a little work
 // behind it:
 //
-// * Work is cut into tiles of 4 KB keys (KB a warp) of one (sequence, key-value
-//   head, block of query heads), numbered in that order over the whole batch.
+// * Work is cut into tiles of 4 x KB keys (KB for each warp) of one (sequence,
+//   key-value head, block of query heads), numbered in that order over the whole batch.
 //   Every CTA takes an equal run of tiles, so ragged lengths, one long sequence
 //   or a thousand short ones load the SMs alike, and nothing about the lengths
 //   has to be known on the host (a captured graph stays valid).
