@@ -358,7 +358,8 @@ int th_rope_append(const th_rope_args* a, void* stream);
  * over keys j < lens[b] (the new token's own key is the last one), with
  * window > 0 only the last `window` of them.  Key j of sequence b is slot
  * j % page_size of page table[b, j / page_size].  Query head h reads
- * key-value head h / (hq/hkv).  lens[b] <= 0 gives zeros (and lse = -inf).
+ * key-value head h / (hq/hkv).  lens[b] <= 0 gives zeros (and lse = -inf),
+ * and so does a head whose scores are all -inf.
  * lse, when given, is log sum_j exp(s_j), fp32 [batch, hq] contiguous.
  * Scores, maxima, sums and accumulators are fp32.  A page id out of range,
  * or a length beyond table_cols * page_size, sets TH_DEVERR_BAD_ARG and

@@ -379,6 +379,23 @@ def test_attention_nan_key_under_a_cap(L, dtype):
     check_attend(L, q, kp, vp, table, n, softcap=20.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_scores_of_minus_infinity(L, dtype):
+    """Keys that a caller has written off with -inf take no weight; a head with nothing else gives zeros."""
+    kp, vp, table, n = cached([70, 33], 1, 64, 16, dtype)
+    q = torch.zeros(2, 4, 64, dtype=dtype, device="cuda")
+    q[:, :, 3] = 1.0
+    kp[table[0, 1], 0, :, 3] = float("-inf")  # keys 16 to 31 of the first sequence
+    kp[table[1, :3].long(), 0, :, 3] = float("-inf")  # all of the second's
+    lse = torch.empty(2, 4, device="cuda")
+    out = L.paged_attention(q, kp, vp, table, n, lse=lse)
+    keep = torch.cat((torch.arange(16), torch.arange(32, 70))).cuda()
+    x = kp[table[0, keep // 16].long(), 0, keep % 16, 3].double() * 0.125
+    want = torch.softmax(x, 0) @ vp[table[0, keep // 16].long(), 0, keep % 16].double()
+    assert rel_l2(out[0], want.expand(4, 64)) <= U[dtype] + 1e-5
+    assert bool((out[1] == 0).all()) and bool((lse[1] == float("-inf")).all())
+
+
 def test_attention_one_workspace_for_several_kinds(L):
     """Calls of other head sizes, groups and types may use one workspace in turn, if it is large enough for each."""
     cases = []
